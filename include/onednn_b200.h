@@ -101,7 +101,10 @@ typedef enum {
 
 typedef enum {
     dnnl_undefined_primitive = 0, dnnl_reorder = 1, dnnl_sum = 4, dnnl_eltwise = 7,
-    dnnl_inner_product = 10, dnnl_binary = 13, dnnl_matmul = 14, dnnl_prelu = 18
+    dnnl_inner_product = 10, dnnl_binary = 13, dnnl_matmul = 14, dnnl_prelu = 18,
+    /* extensions, no counterparts in the reference (values outside its range) */
+    dnnl_b200_rms_norm = 0x4001, dnnl_b200_kv_cache_append = 0x4002, dnnl_b200_kv_cache_read = 0x4003,
+    dnnl_b200_kv_cache_attention = 0x4004
 } dnnl_primitive_kind_t;
 
 typedef enum { dnnl_prop_kind_undef = 0, dnnl_forward_training = 64, dnnl_forward_inference = 96 } dnnl_prop_kind_t;
@@ -150,9 +153,11 @@ typedef enum { dnnl_profiling_data_kind_undef = 0, dnnl_profiling_data_kind_time
 #define DNNL_ARG_DST_0 17
 #define DNNL_ARG_DST DNNL_ARG_DST_0
 #define DNNL_ARG_TO DNNL_ARG_DST_0
+#define DNNL_ARG_DST_1 18
 #define DNNL_ARG_WEIGHTS_0 33
 #define DNNL_ARG_WEIGHTS DNNL_ARG_WEIGHTS_0
 #define DNNL_ARG_BIAS 41
+#define DNNL_ARG_SCALE 51
 #define DNNL_ARG_SCRATCHPAD 80
 /* Extension (no counterpart in the reference): up to seven more destinations, i = 0 .. 6,
  * given consecutively from 0.  Each is a dnnl_memory with the descriptor of DNNL_ARG_DST
@@ -161,6 +166,14 @@ typedef enum { dnnl_profiling_data_kind_undef = 0, dnnl_profiling_data_kind_time
  * N-split layer's slices reach all GPUs from the matmul's own epilogue.  Implementations
  * that cannot do it return dnnl_unimplemented at execution. */
 #define DNNL_ARG_B200_DST_PEER(i) (3072 + (i))
+/* Extension: the paged 8-bit cache of keys and values (dnnl_b200_kv_cache_* below) */
+#define DNNL_ARG_B200_KEY_CACHE 3200
+#define DNNL_ARG_B200_VALUE_CACHE 3201
+#define DNNL_ARG_B200_KEY_SCALES 3202
+#define DNNL_ARG_B200_VALUE_SCALES 3203
+#define DNNL_ARG_B200_PAGE_TABLE 3204
+#define DNNL_ARG_B200_SEQ_OFFSETS 3205
+#define DNNL_ARG_B200_KV_LENS 3206
 #define DNNL_ARG_ATTR_SCALES 4096
 #define DNNL_ARG_ATTR_ZERO_POINTS 8192
 #define DNNL_ARG_ATTR_MULTIPLE_POST_OP_BASE 32768
@@ -356,6 +369,56 @@ dnnl_status_t DNNL_API dnnl_inner_product_forward_primitive_desc_create(dnnl_pri
 dnnl_status_t DNNL_API dnnl_reorder_primitive_desc_create(dnnl_primitive_desc_t *reorder_primitive_desc,
         const_dnnl_memory_desc_t src_desc, dnnl_engine_t src_engine, const_dnnl_memory_desc_t dst_desc,
         dnnl_engine_t dst_engine, const_dnnl_primitive_attr_t attr);
+/* ---- extensions: the operators around the matmul of a transformer's layer ----------
+ * No counterparts in the reference.  Descriptors are plain (no format_tag::any, no runtime
+ * dims) with a contiguous last dim; every other stride is free.  The attribute may set the
+ * scratchpad mode and nothing else.  A combination that is not built is
+ * dnnl_unimplemented, one that contradicts itself dnnl_invalid_arguments.
+ *
+ * dnnl_b200_rms_norm: dst = h * rsqrt(mean(h^2) + epsilon) * scale over the last dim, with
+ *   h = src + residual added in f32.  Up to DNNL_MAX_NDIMS dims; the leading ones must fold into
+ *   rows of one stride.  src, residual: f32 / bf16 / f16 (each its own); scale_desc: the last
+ *   dim, f32 / bf16 / f16, or NULL; residual_desc: like src, or NULL.  dst f32 / bf16 / f16, or
+ *   s8 / f8_e4m3 quantised with one scale per row, max |row| / 127 or / 448, which the primitive
+ *   WRITES to DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST: f32, one per row -- what a matmul takes as its
+ *   source scales with a mask over rows and one group over K.
+ *   Arguments: DNNL_ARG_SRC, DNNL_ARG_SRC_1 (residual), DNNL_ARG_SCALE; DNNL_ARG_DST,
+ *   DNNL_ARG_DST_1 (h rounded to the residual's type, same descriptor; may be the residual's own memory).
+ *
+ * The cache: keys and values each of one descriptor (pages, heads, tokens per page, dim), s8 or
+ *   f8_e4m3, with one f32 scale per page and head (DNNL_ARG_B200_KEY_SCALES / _VALUE_SCALES,
+ *   dense (pages, heads)).  table_desc (sequences, pages per sequence), s32: where the pages of
+ *   each sequence are.  Rows of the other tensors form a ragged batch: rows
+ *   DNNL_ARG_B200_SEQ_OFFSETS[b] .. [b + 1] - 1 (s32, sequences + 1, rising) are the last tokens of
+ *   sequence b, which has DNNL_ARG_B200_KV_LENS[b] tokens (s32) with them.  Rows outside the
+ *   offsets are left alone, so that descriptors may be larger than a step's batch.  A page
+ *   index outside the cache is never followed: its tokens are left out and the next
+ *   dnnl_stream_wait returns dnnl_runtime_error.
+ *
+ * dnnl_b200_kv_cache_append: keys DNNL_ARG_SRC and values DNNL_ARG_SRC_1, both src_desc (rows, heads,
+ *   dim), f32 / bf16 / f16 -- slices of a matmul's result, say -- are quantised into the cache.  The
+ *   scale of a page grows to what its tokens need, and the codes it held are then rounded again.
+ *   Two sequences of one call may not write the same page.
+ * dnnl_b200_kv_cache_read: the inverse; DNNL_ARG_DST and DNNL_ARG_DST_1 of dst_desc (rows, heads, dim).
+ * dnnl_b200_kv_cache_attention: DNNL_ARG_SRC, the queries (rows, q heads, dim), q heads a multiple
+ *   of the cache's heads, attend to the tokens of their sequence up to their own;
+ *   DNNL_ARG_DST the same dims.  dim at most 256.  softmax_scale multiplies query . key.  A row
+ *   that sees no token is zero.  Different executions of one primitive must not overlap in time
+ *   unless the scratchpad is the user's (DNNL_ARG_SCRATCHPAD); a captured execution has one of its own. */
+dnnl_status_t DNNL_API dnnl_b200_rms_norm_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc,
+        const_dnnl_memory_desc_t scale_desc, const_dnnl_memory_desc_t dst_desc, float epsilon,
+        const_dnnl_primitive_attr_t attr);
+dnnl_status_t DNNL_API dnnl_b200_kv_cache_append_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t cache_desc,
+        const_dnnl_memory_desc_t table_desc, const_dnnl_primitive_attr_t attr);
+dnnl_status_t DNNL_API dnnl_b200_kv_cache_read_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t cache_desc, const_dnnl_memory_desc_t dst_desc,
+        const_dnnl_memory_desc_t table_desc, const_dnnl_primitive_attr_t attr);
+dnnl_status_t DNNL_API dnnl_b200_kv_cache_attention_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
+        dnnl_engine_t engine, const_dnnl_memory_desc_t query_desc, const_dnnl_memory_desc_t cache_desc,
+        const_dnnl_memory_desc_t dst_desc, const_dnnl_memory_desc_t table_desc, float softmax_scale,
+        const_dnnl_primitive_attr_t attr);
 dnnl_status_t DNNL_API dnnl_primitive_desc_next_impl(dnnl_primitive_desc_t primitive_desc);
 dnnl_status_t DNNL_API dnnl_primitive_desc_clone(dnnl_primitive_desc_t *primitive_desc,
         const_dnnl_primitive_desc_t existing);

@@ -276,6 +276,89 @@ B200_API int b200_colsum_launch(const void *wei, int32_t wei_dt, int64_t K, int6
 B200_API int b200_gather_columns_launch(const void *staged, void *dst, int64_t M, int64_t N, int32_t parts,
         int32_t elem_bytes, b200_stream_t stream);
 
+/* ---- the operators around the matmul of a transformer's layer ---------------- */
+
+/* Root-mean-square norm of src + residual, row by row, with an 8-bit destination quantised
+ * on the way.  For row m of `cols` elements, every step in f32:
+ *   h[n] = src[m][n] + residual[m][n];  sum[m][n] = h[n] rounded to the residual's type
+ *   y[n] = h[n] * rsqrt(mean(h^2) + epsilon) * gamma[n]
+ *   s8 / f8_e4m3 dst: row_scale[m] = max(max_n |y[n]| * (1 / peak), 2^-126), peak = 127 or 448;
+ *                     dst[m][n] = y[n] * (1 / row_scale[m]), rounded to nearest even, at most
+ *                     the peak in magnitude
+ *   other dst:        dst[m][n] = y[n] rounded to its type
+ * Rows are contiguous inside, src_s0 etc. apart (elements).  residual and sum may be the same
+ * buffer, and sum may be src's; NULL residual: h = src and nothing is stored to sum.  src and
+ * residual are f32 / bf16 / f16, gamma f32 / bf16 / f16 or NULL.  A NaN in a row makes its
+ * outputs NaN (8-bit: the row's scale).  No counterpart in the reference. */
+typedef struct {
+    int64_t rows, cols;
+    const void *src; int32_t src_dt; int32_t reserved0; int64_t src_s0;
+    const void *residual; void *sum; int32_t residual_dt; int32_t reserved1; int64_t residual_s0, sum_s0;
+    const void *gamma; int32_t gamma_dt; int32_t reserved2;
+    void *dst; int32_t dst_dt; int32_t reserved3; int64_t dst_s0;
+    float *row_scale;
+    float epsilon; int32_t reserved4;
+} b200_rms_norm_params_t;
+
+B200_API int b200_rms_norm_launch(const b200_rms_norm_params_t *p, b200_stream_t stream);
+
+/* A paged cache of keys and values in 8 bits, and a ragged batch over it.  Token `at` of
+ * sequence b is slot at % page of the page table[b * table_s0 + at / page]; its head h is `dim`
+ * contiguous codes at key + page index * s_page + h * s_head + slot * s_slot (and the same for
+ * value), which stand for code * scale[page index * heads + h].
+ * Rows offsets[b] .. offsets[b + 1] - 1 of the other tensors belong to sequence b and stand for
+ * its last tokens: with n = offsets[b + 1] - offsets[b], row offsets[b] + i is token
+ * lens[b] - n + i.  Rows of no sequence are neither read nor written.
+ * A page index outside 0 .. pages - 1, or a token beyond the table, is never accessed: the
+ * kernels OR B200_STATUS_BAD_PAGE into *status and carry on without that token. */
+#define B200_STATUS_BAD_PAGE 0x40000000u
+typedef struct {
+    void *key, *value;
+    float *key_scale, *value_scale;
+    int32_t dt; int32_t reserved0;         /* B200_DT_S8 or B200_DT_F8_E4M3 */
+    int64_t pages, heads, page, dim;
+    int64_t s_page, s_head, s_slot;        /* bytes, the same for key and value */
+    const int32_t *table; int64_t table_s0, table_cols;
+    const int32_t *offsets, *lens; int64_t seqs;
+    uint32_t *status;
+} b200_kv_cache_t;
+
+/* Rows of keys and values, element strides s_row and s_head, contiguous inside a head: new
+ * tokens quantised into the cache (append), or tokens of the cache read back (read).
+ *
+ * append: a page's scale is what its tokens need, max |x| * (1 / peak) with peak 127 (s8) or
+ * 448 (f8_e4m3), at least 2^-126.  Tokens that a page held before (slots below the first new
+ * one) keep it from shrinking: scale = max(old, needed), and where it grew their codes are
+ * rounded again, code * (old / scale).  New codes are x * (1 / scale), rounded to nearest even
+ * and held to +-peak.  Infinities do not count for the scale and become +-peak, NaN becomes 0.
+ * Sequences of one call must not write the same page.
+ * read: code * scale, rounded once to the rows' type; rows of tokens before the sequence's
+ * first or in a bad page are zero.  No counterparts in the reference. */
+typedef struct {
+    b200_kv_cache_t cache;
+    void *key, *value; int32_t dt; int32_t reserved0;
+    int64_t rows, s_row, s_head;
+} b200_kv_rows_params_t;
+
+B200_API int b200_kv_append_launch(const b200_kv_rows_params_t *p, b200_stream_t stream);
+B200_API int b200_kv_read_launch(const b200_kv_rows_params_t *p, b200_stream_t stream);
+
+/* Attention of each sequence's last tokens over its cache:
+ *   dst[row][j] = sum_t p[t] * v[t] / sum_t p[t],  p[t] = exp(scale * q[row][j] . k[t])
+ * over the tokens t up to the row's own, with the keys and values of head j / (q_heads / heads).
+ * A row that sees no token is zero.  Sums, maxima and exponentials in f32. */
+typedef struct {
+    b200_kv_cache_t cache;
+    const void *query; int32_t query_dt; int32_t reserved0; int64_t query_s0, query_s1;
+    void *dst; int32_t dst_dt; int32_t reserved1; int64_t dst_s0, dst_s1;
+    int64_t rows, q_heads;
+    float scale; int32_t sm_count;
+    void *scratch; size_t scratch_bytes;
+} b200_kv_attention_params_t;
+
+/* any dim up to 256, strides and alignment; query and dst f32 / bf16 / f16 */
+B200_API int b200_kv_attention_generic_launch(const b200_kv_attention_params_t *p, b200_stream_t stream);
+
 /* ---- utilities ----------------------------------------------------------- */
 
 /* Test hook for the bounded-wait mechanism every kernel here uses: one warp polls an

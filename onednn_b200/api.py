@@ -24,9 +24,13 @@ STATUS = {0: "success", 1: "out_of_memory", 2: "invalid_arguments", 3: "unimplem
 
 # argument indices (dnnl_types.h:2471-2700 in the reference)
 ARG_SRC, ARG_SRC_1, ARG_DST, ARG_WEIGHTS, ARG_BIAS = 1, 2, 17, 33, 41
+ARG_DST_1, ARG_SCALE = 18, 51
 ARG_FROM, ARG_TO, ARG_SCRATCHPAD = 1, 17, 80
 ARG_ATTR_SCALES, ARG_ATTR_ZERO_POINTS, ARG_ATTR_MULTIPLE_POST_OP_BASE = 4096, 8192, 32768
 ARG_B200_DST_PEER0 = 3072  # extension: mirrors of dst in other GPUs' memory, up to seven
+# extension: the paged 8-bit cache of keys and values
+ARG_B200_KEY_CACHE, ARG_B200_VALUE_CACHE, ARG_B200_KEY_SCALES, ARG_B200_VALUE_SCALES = 3200, 3201, 3202, 3203
+ARG_B200_PAGE_TABLE, ARG_B200_SEQ_OFFSETS, ARG_B200_KV_LENS = 3204, 3205, 3206
 TAG_ANY, TAG_A, TAG_AB, TAG_BA, TAG_ABC = 1, 2, 3, 14, 4
 GPU = 2
 QUERY_IMPL_INFO_STR, QUERY_SRC_MD, QUERY_WEIGHTS_MD, QUERY_DST_MD, QUERY_SCRATCHPAD_MD, QUERY_EXEC_ARG_MD = \
@@ -338,6 +342,67 @@ def reorder_primitive_desc(src_engine, src_md, dst_engine, dst_md, attr=None):
     return PrimitiveDesc(h, dst_engine)
 
 
+def _handle(md):
+    return md.h if md is not None else None
+
+
+def rms_norm_primitive_desc(engine, src_md, dst_md, epsilon, scale_md=None, residual_md=None, attr=None):
+    """dst = h * rsqrt(mean(h^2) + epsilon) * scale over the last dim, h = src + residual.
+
+    An s8 or f8_e4m3 ``dst`` is quantised with one scale per row, which the primitive writes to
+    ``ARG_ATTR_SCALES | ARG_DST`` (f32, one per row): what a matmul takes as its per-row source scales.
+    Arguments: ARG_SRC, ARG_SRC_1 (residual), ARG_SCALE; ARG_DST, ARG_DST_1 (h in the residual's type, which
+    may be the residual's own memory)."""
+    h = C.c_void_p()
+    _ck(lib().dnnl_b200_rms_norm_primitive_desc_create(
+        C.byref(h), engine.h, src_md.h, _handle(residual_md), _handle(scale_md), dst_md.h, C.c_float(epsilon),
+        _handle(attr)), "rms_norm_primitive_desc_create")
+    return PrimitiveDesc(h, engine)
+
+
+def kv_cache_append_primitive_desc(engine, src_md, cache_md, table_md, attr=None):
+    """Quantise new keys (ARG_SRC) and values (ARG_SRC_1), both ``src_md`` = (rows, heads, dim), into a paged cache.
+
+    ``cache_md`` = (pages, heads, tokens per page, dim), s8 or f8_e4m3, describes ARG_B200_KEY_CACHE and
+    ARG_B200_VALUE_CACHE; ARG_B200_KEY_SCALES and ARG_B200_VALUE_SCALES are f32 (pages, heads).  ``table_md`` =
+    (sequences, pages per sequence), s32: ARG_B200_PAGE_TABLE.  Rows ARG_B200_SEQ_OFFSETS[b] .. [b + 1] - 1 are the last
+    tokens of sequence b, which has ARG_B200_KV_LENS[b] tokens with them (both s32)."""
+    h = C.c_void_p()
+    _ck(lib().dnnl_b200_kv_cache_append_primitive_desc_create(C.byref(h), engine.h, src_md.h, cache_md.h, table_md.h,
+                                                              _handle(attr)), "kv_cache_append_primitive_desc_create")
+    return PrimitiveDesc(h, engine)
+
+
+def kv_cache_read_primitive_desc(engine, cache_md, dst_md, table_md, attr=None):
+    """Tokens of a paged cache back as rows: keys to ARG_DST, values to ARG_DST_1, both ``dst_md`` = (rows, heads, dim).
+    The cache's arguments as for :func:`kv_cache_append_primitive_desc`."""
+    h = C.c_void_p()
+    _ck(lib().dnnl_b200_kv_cache_read_primitive_desc_create(C.byref(h), engine.h, cache_md.h, dst_md.h, table_md.h,
+                                                            _handle(attr)), "kv_cache_read_primitive_desc_create")
+    return PrimitiveDesc(h, engine)
+
+
+def kv_cache_attention_primitive_desc(engine, query_md, cache_md, dst_md, table_md, softmax_scale, attr=None):
+    """Attention of the last tokens of every sequence (ARG_SRC = (rows, q heads, dim), to ARG_DST) over its tokens in
+    the paged cache up to their own; q heads a multiple of the cache's heads."""
+    h = C.c_void_p()
+    _ck(lib().dnnl_b200_kv_cache_attention_primitive_desc_create(
+        C.byref(h), engine.h, query_md.h, cache_md.h, dst_md.h, table_md.h, C.c_float(softmax_scale), _handle(attr)),
+        "kv_cache_attention_primitive_desc_create")
+    return PrimitiveDesc(h, engine)
+
+
+class ExecArgs:
+    """Execution arguments laid out once, for a primitive that runs on the same memory objects many times."""
+
+    def __init__(self, args):
+        self._keep = list(args.values())
+        self.count = len(args)
+        self.array = (ExecArg * len(args))()
+        for i, (k, m) in enumerate(args.items()):
+            self.array[i].arg, self.array[i].memory = k, m.h
+
+
 class Primitive:
     def __init__(self, pd):
         self.pd = pd
@@ -345,11 +410,10 @@ class Primitive:
         _ck(lib().dnnl_primitive_create(C.byref(self.h), pd.h), "primitive_create")
 
     def execute(self, stream, args):
-        """args: {arg index: Memory}"""
-        arr = (ExecArg * len(args))()
-        for i, (k, m) in enumerate(args.items()):
-            arr[i].arg, arr[i].memory = k, m.h
-        _ck(lib().dnnl_primitive_execute(self.h, stream.h, len(args), arr), "primitive_execute")
+        """args: {arg index: Memory}, or the same as :class:`ExecArgs`"""
+        if not isinstance(args, ExecArgs):
+            args = ExecArgs(args)
+        _ck(lib().dnnl_primitive_execute(self.h, stream.h, args.count, args.array), "primitive_execute")
 
     def __del__(self, _destroy=_destroy):
         _destroy(self, "dnnl_primitive_destroy")

@@ -210,6 +210,11 @@ struct dnnl_primitive_desc {
     // kind == dnnl_inner_product: `inner` is the matmul it runs as; weights / bias keep the
     // descriptors the caller gave, (OC, IC) and (OC)
     bool ip = false;
+    // the extension kinds (layer_ops.cpp): the descriptor of every execution argument, the epsilon
+    // or softmax scale, and the counts that the queries report
+    std::map<int, dnnl_memory_desc> ext_args;
+    float ext_param = 0.f;
+    int ext_inputs = 0, ext_outputs = 0;
 
     int64_t M() const { return dst.dims[dst.ndims - 2]; }
     int64_t N() const { return dst.dims[dst.ndims - 1]; }
@@ -251,6 +256,10 @@ dnnl_status_t matmul_validate(const dnnl_memory_desc &src, const dnnl_memory_des
 dnnl_status_t matmul_select_impl(dnnl_primitive_desc *pd, int first);
 dnnl_status_t matmul_execute(const dnnl_primitive *prim, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args);
 dnnl_status_t reorder_execute(const dnnl_primitive *prim, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args);
+// ---- the operators around the matmul (layer_ops.cpp) ----
+bool is_ext_kind(int kind);
+const char *ext_kind_name(int kind);
+dnnl_status_t ext_execute(const dnnl_primitive *prim, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args);
 // ---- host engine (host_engine.cpp) ----
 dnnl_status_t host_reorder_pd_create(dnnl_primitive_desc_t *out, const dnnl_memory_desc &s, dnnl_engine *se,
         const dnnl_memory_desc &d, dnnl_engine *de, const dnnl_primitive_attr *attr);

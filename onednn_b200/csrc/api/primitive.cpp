@@ -361,6 +361,10 @@ dnnl_status_t dnnl_primitive_desc_destroy(dnnl_primitive_desc_t pd) {
 // the descriptor a runtime argument must have (reference: primitive_desc_t::arg_md
 // and matmul_pd_t::arg_md, src/common/matmul_pd.hpp:73-95)
 static const dnnl_memory_desc *arg_md(const dnnl_primitive_desc *pd, int arg) {
+    if (is_ext_kind(pd->kind) && arg != DNNL_ARG_SCRATCHPAD) {
+        auto it = pd->ext_args.find(arg);
+        return it == pd->ext_args.end() ? &pd->zero_md : &it->second;
+    }
     if (pd->kind == dnnl_reorder) {
         if (arg == DNNL_ARG_FROM) return &pd->src;
         if (arg == DNNL_ARG_TO) return &pd->dst;
@@ -449,7 +453,8 @@ dnnl_status_t dnnl_primitive_desc_query(const_dnnl_primitive_desc_t pd, dnnl_que
         case dnnl_query_primitive_kind: *(dnnl_primitive_kind_t *)result = pd->kind; break;
         case dnnl_query_num_of_inputs_s32: {
             int n = 2;
-            if (pd->kind == dnnl_reorder) n = 1;
+            if (is_ext_kind(pd->kind)) n = pd->ext_inputs;
+            else if (pd->kind == dnnl_reorder) n = 1;
             else {
                 if (pd->bias.ndims) ++n;
                 for (auto &e : pd->attr.post_ops.entries)
@@ -459,7 +464,7 @@ dnnl_status_t dnnl_primitive_desc_query(const_dnnl_primitive_desc_t pd, dnnl_que
             }
             *(int *)result = n;
         } break;
-        case dnnl_query_num_of_outputs_s32: *(int *)result = 1; break;
+        case dnnl_query_num_of_outputs_s32: *(int *)result = is_ext_kind(pd->kind) ? pd->ext_outputs : 1; break;
         case dnnl_query_time_estimate_f64: *(double *)result = 0.0; break;
         case dnnl_query_memory_consumption_s64: *(int64_t *)result = (int64_t)pd->scratchpad.size_bytes(); break;
         case dnnl_query_impl_info_str: *(const char **)result = pd->impl_str.c_str(); break;
@@ -532,6 +537,11 @@ std::string make_key(const dnnl_primitive_desc *pd) {
     key_md(k, pd->wei);
     key_md(k, pd->bias);
     key_md(k, pd->dst);
+    for (const auto &e : pd->ext_args) {
+        k.append((const char *)&e.first, sizeof(int));
+        key_md(k, e.second);
+    }
+    k.append((const char *)&pd->ext_param, sizeof(float));
     k += pd->attr.str();
     char buf[64];
     for (auto &e : pd->attr.post_ops.entries) { // exact float parameters (str() rounds them)
@@ -674,6 +684,7 @@ dnnl_status_t dnnl_primitive_execute(const_dnnl_primitive_t primitive, dnnl_stre
     }
     dnnl_status_t st = pd->kind == dnnl_matmul ? matmul_execute(primitive, stream, m)
             : pd->kind == dnnl_inner_product   ? inner_product_execute(primitive, stream, m)
+            : is_ext_kind(pd->kind)            ? ext_execute(primitive, stream, m)
                                                : reorder_execute(primitive, stream, m);
     if (st != dnnl_success && st != dnnl_invalid_arguments && st != dnnl_unimplemented)
         g_scratch_epoch.fetch_add(1); // a launch sequence may have stopped half way

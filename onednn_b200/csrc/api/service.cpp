@@ -78,7 +78,7 @@ static void line(const char *what, const dnnl_primitive_desc *pd, double ms, con
         mds = md_verbose("src", pd->src) + " " + md_verbose("dst", pd->dst);
     }
     std::printf("onednn_verbose,v1,primitive,%s%s,gpu:%d,%s,%s,undef,%s,%s,,%s,%g\n", what, extra, pd->engine->device,
-            pd->kind == dnnl_matmul ? "matmul" : "reorder", pd->impl_str.c_str(), mds.c_str(), pd->attr.str().c_str(),
+            pd->kind == dnnl_matmul ? "matmul" : is_ext_kind(pd->kind) ? ext_kind_name(pd->kind) : "reorder", pd->impl_str.c_str(), mds.c_str(), pd->attr.str().c_str(),
             problem(pd).c_str(), ms);
     std::fflush(stdout);
 }
