@@ -353,11 +353,19 @@ typedef struct {
     void *dst; int32_t dst_dt; int32_t reserved1; int64_t dst_s0, dst_s1;
     int64_t rows, q_heads;
     float scale; int32_t sm_count;
+    /* of the kernels with a _scratch_bytes function; scratch_zeroed as in b200_matmul_params_t */
     void *scratch; size_t scratch_bytes;
+    int32_t scratch_zeroed; int32_t reserved2;
 } b200_kv_attention_params_t;
 
 /* any dim up to 256, strides and alignment; query and dst f32 / bf16 / f16 */
 B200_API int b200_kv_attention_generic_launch(const b200_kv_attention_params_t *p, b200_stream_t stream);
+
+/* Few query rows per key head, on mma.sync: dim a multiple of 16 up to 256, 16-byte aligned rows, query and
+ * dst bf16 / f16.  _supported looks at types, sizes, strides and pointers (NULL counts as aligned). */
+B200_API int b200_kv_attention_mma_supported(const b200_kv_attention_params_t *p);
+B200_API size_t b200_kv_attention_mma_scratch_bytes(const b200_kv_attention_params_t *p);
+B200_API int b200_kv_attention_mma_launch(const b200_kv_attention_params_t *p, b200_stream_t stream);
 
 /* ---- utilities ----------------------------------------------------------- */
 

@@ -73,15 +73,19 @@ dnnl_status_t dnnl_engine_create(dnnl_engine_t *engine, dnnl_engine_kind_t kind,
         }
         return dnnl_invalid_arguments;
     }
-    cudaDeviceProp prop;
-    if (cudaGetDeviceProperties(&prop, (int)index) != cudaSuccess) return dnnl_runtime_error;
+    // single attributes: the whole property block takes a millisecond to fill
+    int major = 0, minor = 0, sms = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, (int)index) != cudaSuccess
+            || cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, (int)index) != cudaSuccess
+            || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, (int)index) != cudaSuccess)
+        return dnnl_runtime_error;
     // the kernels are sm_100a only
-    if (prop.major != 10) return dnnl_runtime_error;
+    if (major != 10) return dnnl_runtime_error;
     dnnl_engine *e = new dnnl_engine();
     e->device = (int)index;
-    e->sm_major = prop.major;
-    e->sm_minor = prop.minor;
-    e->sm_count = prop.multiProcessorCount;
+    e->sm_major = major;
+    e->sm_minor = minor;
+    e->sm_count = sms;
     *engine = e;
     return dnnl_success;
 }

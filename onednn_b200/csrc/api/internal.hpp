@@ -259,6 +259,7 @@ dnnl_status_t reorder_execute(const dnnl_primitive *prim, dnnl_stream *stream, c
 // ---- the operators around the matmul (layer_ops.cpp) ----
 bool is_ext_kind(int kind);
 const char *ext_kind_name(int kind);
+dnnl_status_t ext_next_impl(dnnl_primitive_desc *pd); // the descriptor stays as it is when there is none
 dnnl_status_t ext_execute(const dnnl_primitive *prim, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args);
 // ---- host engine (host_engine.cpp) ----
 dnnl_status_t host_reorder_pd_create(dnnl_primitive_desc_t *out, const dnnl_memory_desc &s, dnnl_engine *se,

@@ -206,15 +206,38 @@ dnnl_status_t kv_rows_execute(const dnnl_primitive_desc *pd, dnnl_stream *stream
     return status_of(append ? b200_kv_append_launch(&p, stream->cuda_stream) : b200_kv_read_launch(&p, stream->cuda_stream));
 }
 
-dnnl_status_t attention_execute(const dnnl_primitive_desc *pd, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args) {
+// The attention implementations of this engine, in dispatch order.
+struct attention_impl_t {
+    const char *name;
+    int (*supported)(const b200_kv_attention_params_t *);
+    size_t (*scratch_bytes)(const b200_kv_attention_params_t *);
+    int (*launch)(const b200_kv_attention_params_t *, b200_stream_t);
+};
+const attention_impl_t attention_impls[] = {
+        {"cuda:sm100:kv_attention_mma", b200_kv_attention_mma_supported, b200_kv_attention_mma_scratch_bytes,
+                b200_kv_attention_mma_launch},
+        {"cuda:generic", nullptr, nullptr, b200_kv_attention_generic_launch}};
+constexpr int ATTENTION_IMPLS = sizeof(attention_impls) / sizeof(attention_impls[0]);
+
+// what the descriptors say; the pointers stay NULL
+b200_kv_attention_params_t attention_params(const dnnl_primitive_desc *pd) {
     b200_kv_attention_params_t p;
     std::memset(&p, 0, sizeof(p));
-    p.cache = cache_of(pd, stream, args);
-    p.query = at(args, DNNL_ARG_SRC);
+    const dnnl_memory_desc &c = pd->ext_args.at(DNNL_ARG_B200_KEY_CACHE), &t = pd->ext_args.at(DNNL_ARG_B200_PAGE_TABLE);
+    p.cache.dt = c.data_type;
+    p.cache.pages = c.dims[0];
+    p.cache.heads = c.dims[1];
+    p.cache.page = c.dims[2];
+    p.cache.dim = c.dims[3];
+    p.cache.s_page = c.strides[0];
+    p.cache.s_head = c.strides[1];
+    p.cache.s_slot = c.strides[2];
+    p.cache.seqs = t.dims[0];
+    p.cache.table_s0 = t.strides[0];
+    p.cache.table_cols = t.dims[1];
     p.query_dt = pd->src.data_type;
     p.query_s0 = pd->src.strides[0];
     p.query_s1 = pd->src.strides[1];
-    p.dst = at(args, DNNL_ARG_DST);
     p.dst_dt = pd->dst.data_type;
     p.dst_s0 = pd->dst.strides[0];
     p.dst_s1 = pd->dst.strides[1];
@@ -222,7 +245,66 @@ dnnl_status_t attention_execute(const dnnl_primitive_desc *pd, dnnl_stream *stre
     p.q_heads = pd->src.dims[1];
     p.scale = pd->ext_param;
     p.sm_count = pd->engine->sm_count;
-    return status_of(b200_kv_attention_generic_launch(&p, stream->cuda_stream));
+    return p;
+}
+
+// the first implementation from `first` on that takes the problem
+dnnl_status_t attention_select(dnnl_primitive_desc *pd, int first) {
+    b200_kv_attention_params_t p = attention_params(pd);
+    // offset0 moves where the first element is: a pointer of that value stands for it
+    const auto place = [](const dnnl_memory_desc &md) { return (char *)nullptr + md.offset0 * dt_nbits(md.data_type) / 8; };
+    p.query = place(pd->src);
+    p.dst = place(pd->dst);
+    p.cache.key = p.cache.value = place(pd->ext_args.at(DNNL_ARG_B200_KEY_CACHE));
+    for (int i = first; i < ATTENTION_IMPLS; ++i) {
+        const attention_impl_t &impl = attention_impls[i];
+        if (impl.supported && !impl.supported(&p)) continue;
+        pd->impl = i;
+        pd->impl_str = impl.name;
+        pd->scratchpad = dnnl_memory_desc();
+        // sizes only; a descriptor-only engine has no multiprocessors, and nothing to run on
+        const size_t bytes = impl.scratch_bytes ? impl.scratch_bytes(&p) : 0;
+        if (bytes) pd->scratchpad = dense(dnnl_u8, {(int64_t)bytes});
+        return dnnl_success;
+    }
+    return dnnl_unimplemented;
+}
+
+dnnl_status_t attention_execute(const dnnl_primitive *prim, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args) {
+    const dnnl_primitive_desc *pd = prim->pd.get();
+    b200_kv_attention_params_t p = attention_params(pd);
+    p.cache = cache_of(pd, stream, args);
+    p.query = at(args, DNNL_ARG_SRC);
+    p.dst = at(args, DNNL_ARG_DST);
+    const attention_impl_t *impl = &attention_impls[pd->impl];
+    // buffers that start where 16-byte accesses cannot (the descriptors' strides were checked at creation)
+    if (impl->supported && !impl->supported(&p)) impl = &attention_impls[ATTENTION_IMPLS - 1];
+    p.scratch_bytes = impl->scratch_bytes && pd->scratchpad.ndims ? (size_t)pd->scratchpad.dims[0] : 0;
+    if (!p.scratch_bytes) return status_of(impl->launch(&p, stream->cuda_stream));
+
+    const cudaStream_t cs = (cudaStream_t)stream->cuda_stream;
+    if (pd->attr.scratchpad_mode == dnnl_scratchpad_mode_user) {
+        auto it = args.find(DNNL_ARG_SCRATCHPAD);
+        if (it == args.end() || !it->second->handle || it->second->md.size_bytes() < p.scratch_bytes) return dnnl_invalid_arguments;
+        p.scratch = at(args, DNNL_ARG_SCRATCHPAD);
+        return status_of(impl->launch(&p, cs));
+    }
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(cs, &capture) != cudaSuccess) return dnnl_runtime_error;
+    if (capture != cudaStreamCaptureStatusNone) {
+        // a graph may be replayed next to others and to eager executions: it gets memory of its own
+        if (device_alloc_async(&p.scratch, p.scratch_bytes, cs) != cudaSuccess) return dnnl_out_of_memory;
+        const dnnl_status_t st = status_of(impl->launch(&p, cs));
+        if (cudaFreeAsync(p.scratch, cs) != cudaSuccess) return dnnl_runtime_error;
+        return st;
+    }
+    // as for the matmul: zeroed at creation, left zeroed, cleared again after an error
+    p.scratch = prim->lib_scratch;
+    if (!p.scratch) return dnnl_out_of_memory;
+    const uint64_t now = g_scratch_epoch.load();
+    if (prim->scratch_epoch.exchange(now) == now) p.scratch_zeroed = 1;
+    else g_scratch_reclears.fetch_add(1);
+    return status_of(impl->launch(&p, cs));
 }
 
 } // namespace
@@ -240,6 +322,11 @@ const char *ext_kind_name(int kind) {
     }
 }
 
+dnnl_status_t ext_next_impl(dnnl_primitive_desc *pd) {
+    if (pd->kind != dnnl_b200_kv_cache_attention) return dnnl_last_impl_reached; // one implementation
+    return attention_select(pd, pd->impl + 1) == dnnl_success ? dnnl_success : dnnl_last_impl_reached;
+}
+
 dnnl_status_t ext_execute(const dnnl_primitive *prim, dnnl_stream *stream, const std::map<int, dnnl_memory *> &args) {
     const dnnl_primitive_desc *pd = prim->pd.get();
     const dnnl_memory_desc &rows = pd->kind == dnnl_b200_kv_cache_read ? pd->dst : pd->src;
@@ -251,7 +338,7 @@ dnnl_status_t ext_execute(const dnnl_primitive *prim, dnnl_stream *stream, const
     }
     switch (pd->kind) {
         case dnnl_b200_rms_norm: return norm_execute(pd, stream, args);
-        case dnnl_b200_kv_cache_attention: return attention_execute(pd, stream, args);
+        case dnnl_b200_kv_cache_attention: return attention_execute(prim, stream, args);
         default: return kv_rows_execute(pd, stream, args);
     }
 }
@@ -381,7 +468,6 @@ dnnl_status_t dnnl_b200_kv_cache_attention_primitive_desc_create(dnnl_primitive_
     pd->ext_args[DNNL_ARG_DST] = *dst_desc;
     pd->ext_inputs = 8;
     pd->ext_outputs = 1;
-    pd->impl = 0;
-    pd->impl_str = "cuda:generic";
+    if ((st = attention_select(pd.get(), 0)) != dnnl_success) return st;
     return finish(pd, primitive_desc, t0);
 } catch (const std::bad_alloc &) { return dnnl_out_of_memory; }

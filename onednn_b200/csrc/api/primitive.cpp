@@ -329,6 +329,7 @@ dnnl_status_t reorder_execute(const dnnl_primitive *prim, dnnl_stream *stream, c
 
 dnnl_status_t dnnl_primitive_desc_next_impl(dnnl_primitive_desc_t pd) {
     if (!pd) return dnnl_invalid_arguments;
+    if (is_ext_kind(pd->kind)) return ext_next_impl(pd);
     if (pd->kind != dnnl_matmul) return dnnl_last_impl_reached; // reorder, inner product: one implementation
     dnnl_primitive_desc trial = *pd;
     dnnl_status_t st = matmul_select_impl(&trial, pd->impl + 1);
