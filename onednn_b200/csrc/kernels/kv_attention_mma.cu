@@ -24,10 +24,13 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32, UNIT = WARPS * STEP;
 
+// blocks per SM
+__host__ __device__ constexpr int blocks_of(int dp, int nb) { return dp == 64 ? (nb == 1 ? 4 : nb == 2 ? 3 : 2) : dp == 128 ? (nb == 1 ? 3 : 2) : 1; }
+
 template <int DP, int NB>
 struct shape_t {
-    static constexpr int STAGES = DP == 64 ? 4 : 3;
-    static constexpr int BLOCKS = DP == 64 && NB < 4 ? 3 : DP <= 128 ? 2 : 1; // per SM
+    static constexpr int BLOCKS = blocks_of(DP, NB);
+    static constexpr int STAGES = DP == 64 ? 3 : BLOCKS == 3 ? 2 : 3;
     static constexpr int ROWS = 8 * NB;
     static constexpr int STAGE = 2 * STEP * DP + 2 * STEP * 4;      // keys, values, their scales
     static constexpr int RING = STAGES * STAGE;
@@ -143,7 +146,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sum) {
     return v;
 }
 
-template <int DP, int NB, bool S8>
+template <int DP, int NB, bool S8, bool RUNS>
 __global__ void __launch_bounds__(THREADS, shape_t<DP, NB>::BLOCKS)
 kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     using S = shape_t<DP, NB>;
@@ -159,6 +162,9 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int heads = (int)c.heads, group = (int)(p.q_heads / c.heads), page = (int)c.page, pieces = (int)c.dim / 16;
     const int64_t capacity = min((int64_t)0x7fffff00, c.table_cols * c.page);
+    // an f16 result shows a weight's rounding to f16: what the rounding left is multiplied too (bf16's own
+    // last rounding is eight times as large)
+    const bool fine = p.dst_dt == B200_DT_F16;
 
     // the whole line, and this block's part of it
     int64_t total = 0;
@@ -242,42 +248,67 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         const int32_t *table = c.table + (int64_t)seq * c.table_s0;
         const uint8_t *keys = (const uint8_t *)c.key + head * c.s_head, *values = (const uint8_t *)c.value + head * c.s_head;
 
-        // ---- copies: the page of this lane's token one step ahead of the copy that needs it
-        int next_page = -1, next_slot = 0;
-        auto look_up = [&](int step) {
-            const int tok = step * STEP + lane;
-            next_page = -1;
-            if (tok < end) {
-                const int j = tok / page;
-                next_slot = tok - j * page;
-                next_page = table[j];
-            }
+        // ---- copies; a lane looks a token's page up one step ahead of the copy that needs it.
+        // Lane l copies piece l % CH of the CH tokens from l / CH * CH on, and its own token's scales.
+        // With RUNS these tokens lie in one page, so that one place serves the lane's copies; without, every token
+        // has a place of its own, from the lane that looked it up.
+        const int lead = RUNS ? lane / CH * CH : lane; // the token of a step that this lane looks up
+        int next_page = -1, next_j, next_slot;
+        const int jump_j = UNIT / page, jump_slot = UNIT - jump_j * page;
+        auto look_up_at = [&](int step) {
+            const int tok = step * STEP + lead;
+            next_j = tok / page;
+            next_slot = tok - next_j * page;
+            next_page = tok < end ? table[next_j] : -1;
+        };
+        auto look_up_next = [&](int step) { // the warp's step after the one looked up before
+            next_j += jump_j;
+            next_slot += jump_slot;
+            if (next_slot >= page) next_slot -= page, ++next_j;
+            next_page = step * STEP + lead < end ? table[next_j] : -1;
         };
         auto copy = [&](int step, int stage) {
             uint8_t *k = ring + stage * S::STAGE, *v = k + STEP * DP;
             float *sk = (float *)(v + STEP * DP), *sv = sk + STEP;
             int64_t place = -1;
-            if (step * STEP + lane < end) {
-                if (next_page >= 0 && next_page < c.pages) {
-                    place = (int64_t)next_page * c.s_page + (int64_t)next_slot * c.s_slot;
-                    const int64_t si = (int64_t)next_page * heads + head;
-                    cp4(smem_u32(sk + lane), c.key_scale + si);
-                    cp4(smem_u32(sv + lane), c.value_scale + si);
-                } else {
-                    flag_bad_page(c);
-                }
+            const int left = end - step * STEP; // tokens of this step and behind
+            if (lead < left) {
+                if (next_page >= 0 && next_page < c.pages) place = (int64_t)next_page * c.s_page + (int64_t)next_slot * c.s_slot;
+                else flag_bad_page(c);
             }
-            if (place < 0) sk[lane] = -1.f, sv[lane] = 0.f; // no such token
-            constexpr int PER = 32 / CH; // tokens per access of the warp
+            if (place >= 0 && lane < left) {
+                const int64_t si = (int64_t)next_page * heads + head;
+                cp4(smem_u32(sk + lane), c.key_scale + si);
+                cp4(smem_u32(sv + lane), c.value_scale + si);
+            } else {
+                sk[lane] = -1.f, sv[lane] = 0.f; // no such token
+            }
             const int cc = lane % CH;
-#pragma unroll
-            for (int i = 0; i < STEP / PER; ++i) {
-                const int r = i * PER + lane / CH;
-                const int64_t from = __shfl_sync(~0u, place, r);
+            if (RUNS) {
                 if (cc < pieces) {
-                    const int64_t o = max(from, (int64_t)0) + cc * 16;
-                    cp16(smem_u32(k + r * DP + key_piece<DP>(r, cc) * 16), keys + o, from >= 0);
-                    cp16(smem_u32(v + r * DP + value_piece<DP>(r, cc) * 16), values + o, from >= 0);
+                    const int64_t o = max(place, (int64_t)0) + cc * 16;
+                    const uint8_t *kf = keys + o, *vf = values + o;
+                    const int ok = place >= 0 ? left - lead : 0;
+                    const uint32_t to = smem_u32(k + lead * DP);
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        const bool take = i < ok;
+                        const int64_t step_over = take ? i * (int64_t)c.s_slot : 0; // no address behind the last page
+                        cp16(to + i * DP + key_piece<DP>(i, cc) * 16, kf + step_over, take);
+                        cp16(to + STEP * DP + i * DP + value_piece<DP>(i, cc) * 16, vf + step_over, take);
+                    }
+                }
+            } else {
+                constexpr int PER = 32 / CH; // tokens per access of the warp
+#pragma unroll
+                for (int i = 0; i < STEP / PER; ++i) {
+                    const int r = i * PER + lane / CH;
+                    const int64_t from = __shfl_sync(~0u, place, r);
+                    if (cc < pieces) {
+                        const int64_t o = max(from, (int64_t)0) + cc * 16;
+                        cp16(smem_u32(k + r * DP + key_piece<DP>(r, cc) * 16), keys + o, from >= 0);
+                        cp16(smem_u32(v + r * DP + value_piece<DP>(r, cc) * 16), values + o, from >= 0);
+                    }
                 }
             }
         };
@@ -286,12 +317,12 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         for (int i = 0; i < S::STAGES - 1; ++i) {
             const int step = first_step + i * WARPS;
             if (step < steps_end) {
-                look_up(step);
+                look_up_at(step);
                 copy(step, i);
             }
             cp_commit();
         }
-        look_up(first_step + (S::STAGES - 1) * WARPS);
+        look_up_at(first_step + (S::STAGES - 1) * WARPS);
 
         // ---- queries: row g of each tile of eight, four neighbouring dims per instruction
         uint32_t q[S::Q_SHARED ? 1 : KS][S::Q_SHARED ? 1 : NB][2];
@@ -423,10 +454,23 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                     for (int h = 0; h < 2; ++h) {
                         float &x = st[i >> 1][nb][(i & 1) * 2 + h];
                         x = x * ks[i] * factor[nb][h];
-                        if (masked && (ks[i] < 0.f || step * STEP + g + 8 * i > limit[nb][h])) x = -INFINITY;
-                        top[nb][h] = fmaxf(top[nb][h], x);
                     }
             }
+            if (masked) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (ks[i] < 0.f || step * STEP + g + 8 * i > limit[nb][h]) st[i >> 1][nb][(i & 1) * 2 + h] = -INFINITY;
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) top[nb][h] = fmaxf(top[nb][h], st[i >> 1][nb][(i & 1) * 2 + h]);
             bool grew = false;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -467,20 +511,26 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             for (int i = 0; i < 4; ++i) vs[i] *= down;
 
             // ---- weights, and the weighted values
-            uint32_t pb[2][NB][2];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w0 = ex2(st[i >> 1][nb][(i & 1) * 2] - m0), w1 = ex2(st[i >> 1][nb][(i & 1) * 2 + 1] - m1);
-                    l[nb][0] += w0;
-                    l[nb][1] += w1;
-                    pb[i >> 1][nb][i & 1] = transposed(pack_f16x2(w0 * vs[i], w1 * vs[i]));
-                }
-            }
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
+                uint32_t pb[NB][2], rest[NB][2];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float w0 = ex2(st[tt][nb][i * 2] - m0), w1 = ex2(st[tt][nb][i * 2 + 1] - m1);
+                        l[nb][0] += w0;
+                        l[nb][1] += w1;
+                        const float p0 = w0 * vs[tt * 2 + i], p1 = w1 * vs[tt * 2 + i];
+                        const uint32_t hi = pack_f16x2(p0, p1);
+                        pb[nb][i] = transposed(hi);
+                        if (fine) {
+                            const float2 had = f16x2_to_f32(hi);
+                            rest[nb][i] = transposed(pack_f16x2(p0 - had.x, p1 - had.y));
+                        }
+                    }
+                }
                 const int r = tt * 16 + 2 * t; // this lane's tokens: r, r + 1, r + 8, r + 9
 #pragma unroll
                 for (int j = 0; j < (DP + 127) / 128; ++j) {
@@ -506,7 +556,10 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                             widen<S8>(prmt(x[0][w], x[1][w], sel), a[0], a[1]);
                             widen<S8>(prmt(x[2][w], x[3][w], sel), a[2], a[3]);
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb) mma(o[j * 8 + w * 2 + h][nb], a, pb[tt][nb]);
+                            for (int nb = 0; nb < NB; ++nb) {
+                                mma(o[j * 8 + w * 2 + h][nb], a, pb[nb]);
+                                if (fine) mma(o[j * 8 + w * 2 + h][nb], a, rest[nb]);
+                            }
                         }
                 }
             }
@@ -514,7 +567,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             const int further = step + (S::STAGES - 1) * WARPS;
             if (further < steps_end) copy(further, stage == 0 ? S::STAGES - 1 : stage - 1);
             cp_commit();
-            look_up(further + WARPS);
+            look_up_next(further + WARPS);
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
         }
         cp_wait<0>();
@@ -596,23 +649,47 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             if (last_part) {
                 __threadfence();
                 const float *first = parts + (size_t)(c0 * 2 + (item_begin == total * c0 / blocks ? 0 : 1)) * part_size;
+                auto part_of = [&](int b) { return b == c0 ? first : parts + (size_t)b * 2 * part_size; };
+                // the parts' weights into shared memory: factor = 2^(m - largest m), then the values eight parts at a time
+                const int n = c1 - c0 + 1;
+                float *fs = (float *)smem; // [n][ROWS]; the host keeps the grid small enough
+                for (int r = warp; r < live; r += WARPS) {
+                    float mm = -INFINITY, ll = 0.f;
+                    for (int b = lane; b < n; b += 32) {
+                        const float mb = __ldcg(part_of(c0 + b) + r);
+                        fs[b * ROWS + r] = mb;
+                        mm = fmaxf(mm, mb);
+                    }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
+                    for (int b = lane; b < n; b += 32) {
+                        const float mb = fs[b * ROWS + r], f = mb == -INFINITY ? 0.f : ex2(mb - mm);
+                        fs[b * ROWS + r] = f;
+                        if (f != 0.f) ll = fmaf(__ldcg(part_of(c0 + b) + ROWS + r), f, ll);
+                    }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(~0u, ll, o);
+                    if (lane == 0) merge_l[0][r] = ll;
+                }
+                __syncthreads();
                 for (int i = tid; i < live * (DP / 4); i += THREADS) {
                     const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
                     if (d >= c.dim) continue;
-                    float mm = -INFINITY, ll = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int b = c0; b <= c1; ++b) {
-                        const float *from = b == c0 ? first : parts + (size_t)b * 2 * part_size;
-                        mm = fmaxf(mm, __ldcg(from + r));
+                    for (int base = 0; base < n; base += 8) {
+                        float4 y[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            if (base + u < n) y[u] = __ldcg((const float4 *)(part_of(c0 + base + u) + 2 * ROWS + r * DP + d));
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            if (base + u >= n) continue;
+                            const float f = fs[(base + u) * ROWS + r];
+                            if (f == 0.f) continue;
+                            x.x = fmaf(y[u].x, f, x.x), x.y = fmaf(y[u].y, f, x.y), x.z = fmaf(y[u].z, f, x.z), x.w = fmaf(y[u].w, f, x.w);
+                        }
                     }
-                    for (int b = c0; b <= c1; ++b) {
-                        const float *from = b == c0 ? first : parts + (size_t)b * 2 * part_size;
-                        const float mb = __ldcg(from + r), f = mb == -INFINITY ? 0.f : ex2(mb - mm);
-                        const float4 y = __ldcg((const float4 *)(from + 2 * ROWS + r * DP + d));
-                        if (f == 0.f) continue;
-                        ll = fmaf(__ldcg(from + ROWS + r), f, ll);
-                        x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
-                    }
+                    const float ll = merge_l[0][r];
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
                     const int idx = tile * ROWS + r;
                     const int64_t off = (int64_t)(s.begin + idx / group) * p.dst_s0 + (int64_t)(head * group + idx % group) * p.dst_s1 + d;
@@ -645,14 +722,17 @@ choice_t choose(const b200_kv_attention_params_t &p) {
     c.dp = p.cache.dim <= 64 ? 64 : p.cache.dim <= 128 ? 128 : 256;
     const int64_t rows = (p.rows + p.cache.seqs - 1) / (p.cache.seqs > 0 ? p.cache.seqs : 1) * (p.q_heads / p.cache.heads);
     c.nb = rows <= 8 ? 1 : rows <= 16 || c.dp == 256 ? 2 : 4;
-    c.blocks = c.dp == 64 && c.nb < 4 ? 3 : c.dp <= 128 ? 2 : 1; // shape_t::BLOCKS
+    c.blocks = blocks_of(c.dp, c.nb);
     return c;
 }
 
-template <int DP, int NB, bool S8>
+template <int DP, int NB, bool S8, bool RUNS>
 int run(const b200_kv_attention_params_t &p, int blocks, cudaStream_t cs) {
     using S = shape_t<DP, NB>;
-    auto kernel = kv_attention_mma_kernel<DP, NB, S8>;
+    auto kernel = kv_attention_mma_kernel<DP, NB, S8, RUNS>;
+    // the joining block keeps a factor per part and row in the rings
+    const int most = (int)(WARPS * S::RING / (S::ROWS * 4));
+    if (blocks > most) blocks = most;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return (int)e;
     kernel<<<blocks, THREADS, S::SMEM, cs>>>(p);
@@ -660,7 +740,11 @@ int run(const b200_kv_attention_params_t &p, int blocks, cudaStream_t cs) {
 }
 template <int DP, int NB>
 int run(const b200_kv_attention_params_t &p, int blocks, cudaStream_t cs) {
-    return p.cache.dt == B200_DT_S8 ? run<DP, NB, true>(p, blocks, cs) : run<DP, NB, false>(p, blocks, cs);
+    // the DP / 16 tokens that a lane copies lie in one page, or may not
+    const bool s8 = p.cache.dt == B200_DT_S8;
+    if (p.cache.page % (DP / 16) == 0)
+        return s8 ? run<DP, NB, true, true>(p, blocks, cs) : run<DP, NB, false, true>(p, blocks, cs);
+    return s8 ? run<DP, NB, true, false>(p, blocks, cs) : run<DP, NB, false, false>(p, blocks, cs);
 }
 
 } // namespace
