@@ -214,6 +214,8 @@ struct attention_impl_t {
     int (*launch)(const b200_kv_attention_params_t *, b200_stream_t);
 };
 const attention_impl_t attention_impls[] = {
+        {"cuda:sm100:kv_attention_tc", b200_kv_attention_tc_supported, b200_kv_attention_tc_scratch_bytes,
+                b200_kv_attention_tc_launch},
         {"cuda:sm100:kv_attention_mma", b200_kv_attention_mma_supported, b200_kv_attention_mma_scratch_bytes,
                 b200_kv_attention_mma_launch},
         {"cuda:generic", nullptr, nullptr, b200_kv_attention_generic_launch}};

@@ -1,11 +1,9 @@
 // Attention over the paged 8-bit cache for few query rows per key head (b200_kv_attention_mma_launch): steps of one
 // token, drafts of a few.  Bound by reading the cache once.
 //
-// A work item is one sequence, one key head and up to 8 * NB query rows (tokens x the query heads that share the key
-// head).  All items' tokens, in units of 128, form one line that is cut into equal parts, one per block, so that ragged
-// batches and single long contexts load every SM alike; blocks derive the cut from the offsets and lengths themselves.
-// An item that was cut is put together by the block that finishes it last, in the order of the parts, so the result does
-// not depend on who is last.
+// Work items of up to 8 * NB query rows are laid out and cut as kv_line.cuh says, so that ragged batches and
+// single long contexts load every SM alike.  An item that was cut is put together by the block that
+// finishes it last, in the order of the parts, so the result does not depend on who is last.
 //
 // Inside a block each of four warps takes every fourth 32 tokens through a ring of its own in shared memory (cp.async,
 // no block barrier in the loop) with its own running maximum, sum and weighted values:
@@ -19,7 +17,7 @@
 // (`ref`); queries are taken to f16 after a power of two per row that brings the largest element to [1, 2).
 #pragma once
 
-#include "kv_cache.cuh"
+#include "kv_line.cuh"
 #include "launch.hpp"
 
 #include <type_traits>
@@ -27,7 +25,10 @@
 namespace b200 {
 namespace kv_mma {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32, UNIT = WARPS * STEP;
+using namespace kv_line;
+
+constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32;
+static_assert(WARPS * STEP == UNIT, "a warp takes one step of each unit");
 
 // blocks per SM
 __host__ __device__ constexpr int blocks_of(int dp, int nb) { return dp == 64 ? (nb == 1 ? 4 : nb == 2 ? 3 : 2) : dp == 128 ? (nb == 1 ? 3 : 2) : 1; }
@@ -46,9 +47,6 @@ struct shape_t {
     static_assert(ROWS * PITCH * 4 <= RING, "the partial values reuse the ring");
 };
 
-// ---- scratch: a counter per block (parts done of the item that begins in its stretch of the line and
-// ends in another's; zero between launches), then per block two partial results ------------------
-__host__ __device__ inline size_t counter_bytes(int blocks) { return ((size_t)blocks * 4 + 255) / 256 * 256; }
 inline size_t part_floats(int dp, int nb) { return (size_t)8 * nb * (dp + 2); }
 
 // ---- small pieces -------------------------------------------------------------------------------
@@ -109,108 +107,21 @@ __device__ __forceinline__ int key_piece(int r, int c) { return DP == 64 ? c : c
 template <int DP>
 __device__ __forceinline__ int value_piece(int r, int c) { return DP == 64 ? c ^ (r & 2) : c ^ (r & 6); }
 
-// ---- the line of work -------------------------------------------------------------------------
-
-struct item_t {
-    int tokens; // that its last row sees
-    int units;
-};
-
-template <int ROWS>
-__device__ __forceinline__ item_t item_of(const seq_t &s, int group, int tile, int64_t capacity) {
-    const int rows = (s.end - s.begin) * group;
-    const int last = (min((tile + 1) * ROWS, rows) - 1) / group; // its newest token
-    const int64_t t = max(0, s.first + last + 1);
-    item_t i;
-    i.tokens = (int)min(t, capacity);
-    i.units = max(1, (i.tokens + UNIT - 1) / UNIT);
-    return i;
-}
-
-// units of one key head of sequence b
-template <int ROWS>
-__device__ __forceinline__ int64_t head_units(const seq_t &s, int group, int64_t capacity) {
-    int64_t n = 0;
-    const int tiles = ((s.end - s.begin) * group + ROWS - 1) / ROWS;
-    for (int i = 0; i < tiles; ++i) n += item_of<ROWS>(s, group, i, capacity).units;
-    return n;
-}
-
-// inclusive sum over the block's threads
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sum) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(~0u, v, o);
-        if (lane >= o) v += u;
-    }
-    __syncthreads();
-    if (lane == 31) warp_sum[warp] = v;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) v += warp_sum[w];
-    return v;
-}
-
 template <int DP, int NB, bool S8, bool RUNS, bool FINE>
 __global__ void __launch_bounds__(THREADS, shape_t<DP, NB>::BLOCKS)
 kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     using S = shape_t<DP, NB>;
     constexpr int ROWS = S::ROWS, KS = DP / 16, CH = DP / 16, MT = DP / 16;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t warp_sum[WARPS];
-    __shared__ int64_t found_rest;
-    __shared__ int found_seq;
+    __shared__ int64_t line_words[34];
     __shared__ float merge_m[WARPS][ROWS], merge_l[WARPS][ROWS];
     __shared__ bool last_part;
 
     const b200_kv_cache_t &c = p.cache;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int heads = (int)c.heads, group = (int)(p.q_heads / c.heads), page = (int)c.page, pieces = (int)c.dim / 16;
-    const int64_t capacity = min((int64_t)0x7fffff00, c.table_cols * c.page);
-
-    // the whole line, and this block's part of it
-    int64_t total = 0;
-    for (int base = 0; base < c.seqs; base += THREADS) {
-        const int b = base + tid;
-        int64_t n = 0;
-        if (b < c.seqs) n = head_units<ROWS>(load_seq(c, b, p.rows), group, capacity) * heads;
-        n = block_scan(n, warp_sum);
-        if (tid == THREADS - 1) found_rest = n;
-        __syncthreads();
-        total += found_rest;
-    }
-    // no part is empty
-    const int blocks = (int)min((int64_t)gridDim.x, total);
-    if (blockIdx.x >= blocks) return;
-    int64_t at = total * blockIdx.x / blocks;
-    const int64_t stop = total * (blockIdx.x + 1) / blocks;
-
-    // the sequence that the part begins in, and the units before it
-    int seq = 0;
-    int64_t seq_begin = 0;
-    for (int base = 0; base < c.seqs; base += THREADS) {
-        const int b = base + tid;
-        int64_t n = 0;
-        if (b < c.seqs) n = head_units<ROWS>(load_seq(c, b, p.rows), group, capacity) * heads;
-        const int64_t upto = seq_begin + block_scan(n, warp_sum);
-        __syncthreads();
-        if (tid == 0) found_seq = -1;
-        __syncthreads();
-        if (upto > at && upto - n <= at) {
-            found_seq = b;
-            found_rest = upto - n;
-        }
-        if (tid == THREADS - 1) warp_sum[0] = upto;
-        __syncthreads();
-        if (found_seq >= 0) {
-            seq = found_seq;
-            seq_begin = found_rest;
-            break;
-        }
-        seq_begin = warp_sum[0];
-        __syncthreads();
-    }
-
+    part_t line;
+    if (!begin_part<ROWS>(p, line, line_words)) return;
+    const int heads = line.heads, group = line.group, page = (int)c.page, pieces = (int)c.dim / 16;
     uint8_t *ring = smem + warp * S::RING;
     uint2 *q_shared = (uint2 *)(smem + WARPS * S::RING);
     // pieces behind dim stay zero: no copy writes them
@@ -220,32 +131,18 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     }
 
     uint32_t *counters = (uint32_t *)p.scratch;
-    float *parts = (float *)((char *)p.scratch + counter_bytes(blocks));
+    float *parts = (float *)((char *)p.scratch + counter_bytes(gridDim.x));
     constexpr size_t part_size = (size_t)ROWS * (DP + 2); // part_floats()
-    const int64_t my_begin = at;
-
-    while (at < stop) {
-        // ---- the item at `at`
-        seq_t s = load_seq(c, seq, p.rows);
-        int64_t per_head = head_units<ROWS>(s, group, capacity);
-        while (at - seq_begin >= per_head * heads) {
-            seq_begin += per_head * heads;
-            ++seq;
-            s = load_seq(c, seq, p.rows);
-            per_head = head_units<ROWS>(s, group, capacity);
-        }
-        const int head = (int)((at - seq_begin) / per_head);
-        int64_t item_begin = seq_begin + head * per_head;
-        int tile = 0;
-        item_t item = item_of<ROWS>(s, group, 0, capacity);
-        while (at - item_begin >= item.units) {
-            item_begin += item.units;
-            item = item_of<ROWS>(s, group, ++tile, capacity);
-        }
-        const int u0 = (int)(at - item_begin), u1 = (int)min((int64_t)item.units, stop - item_begin);
+    int64_t at = line.begin;
+    while (at < line.stop) {
+        const place_t place_at = find_item<ROWS>(p, line, at);
+        const item_t item = place_at.item;
+        const int head = place_at.head, tile = place_at.tile, seq = line.seq;
+        const seq_t s = line.s;
+        const int u0 = (int)(at - place_at.item_begin), u1 = (int)min((int64_t)item.units, line.stop - place_at.item_begin);
         const int rows = (s.end - s.begin) * group - tile * ROWS; // that exist from here on
         const int end = min(u1 * UNIT, item.tokens);
-        if (tid == 0 && u0 == 0 && (int64_t)s.first + (s.end - s.begin) > capacity) flag_bad_page(c);
+        if (tid == 0 && u0 == 0 && (int64_t)s.first + (s.end - s.begin) > line.capacity) flag_bad_page(c);
 
         const int32_t *table = c.table + (int64_t)seq * c.table_s0;
         const uint8_t *keys = (const uint8_t *)c.key + head * c.s_head, *values = (const uint8_t *)c.value + head * c.s_head;
@@ -614,7 +511,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         }
         __syncthreads();
         const bool whole = u0 == 0 && u1 == item.units;
-        float *part = parts + (size_t)(blockIdx.x * 2 + (at == my_begin ? 0 : 1)) * part_size;
+        float *part = parts + (size_t)(blockIdx.x * 2 + (at == line.begin ? 0 : 1)) * part_size;
         const int live = min(rows, ROWS);
         for (int i = tid; i < live * (DP / 4); i += THREADS) {
             const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
@@ -647,14 +544,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
 
         // ---- an item in several parts: the last block to finish one puts them together
         if (!whole) {
-            // the blocks that hold its first and last unit
-            auto owner = [&](int64_t u) {
-                int64_t o = u * blocks / total; // total * o / blocks <= u, or nearly
-                while (total * (o + 1) / blocks <= u) ++o;
-                while (total * o / blocks > u) --o;
-                return (int)o;
-            };
-            const int c0 = owner(item_begin), c1 = owner(item_begin + item.units - 1);
+            const int c0 = owner(line, place_at.item_begin), c1 = owner(line, place_at.item_begin + item.units - 1);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -665,8 +555,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             __syncthreads();
             if (last_part) {
                 __threadfence();
-                const float *first = parts + (size_t)(c0 * 2 + (item_begin == total * c0 / blocks ? 0 : 1)) * part_size;
-                auto part_of = [&](int b) { return b == c0 ? first : parts + (size_t)b * 2 * part_size; };
+                auto part_of = [&](int b) { return parts + part_index(line, place_at.item_begin, c0, b) * part_size; };
                 // the parts' weights into shared memory: factor = 2^(m - largest m), then the values eight parts at a time
                 const int n = c1 - c0 + 1;
                 float *fs = (float *)smem; // [n][ROWS]; the host keeps the grid small enough
@@ -722,7 +611,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             for (int i = tid; i < WARPS * S::RING / 16; i += THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
         }
-        at = item_begin + u1;
+        at = place_at.item_begin + u1;
     }
 }
 

@@ -1,0 +1,162 @@
+// How the attention kernels divide a ragged batch among the SMs.
+//
+// An item is one sequence, one key head and ROWS query rows (tokens x the query heads of the key head); it costs its
+// tokens, in units of 128.  All items side by side -- sequence, head, rows -- form one line of units, which is cut into
+// equal parts, one per block, wherever that falls.  The host knows neither offsets nor lengths, so every
+// block derives the line itself, in two short scans over the sequences.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace b200 {
+namespace kv_line {
+
+constexpr int UNIT = 128;
+
+struct item_t {
+    int tokens; // that its last row sees
+    int units;  // one at least: rows that see nothing are still written
+};
+
+template <int ROWS>
+__device__ __forceinline__ item_t item_of(const seq_t &s, int group, int tile, int64_t capacity) {
+    const int rows = (s.end - s.begin) * group;
+    const int last = (min((tile + 1) * ROWS, rows) - 1) / group; // its newest token
+    const int64_t t = max(0, s.first + last + 1);
+    item_t i;
+    i.tokens = (int)min(t, capacity);
+    i.units = max(1, (i.tokens + UNIT - 1) / UNIT);
+    return i;
+}
+
+// units of one key head of a sequence
+template <int ROWS>
+__device__ __forceinline__ int64_t head_units(const seq_t &s, int group, int64_t capacity) {
+    int64_t n = 0;
+    const int tiles = ((s.end - s.begin) * group + ROWS - 1) / ROWS;
+    for (int i = 0; i < tiles; ++i) n += item_of<ROWS>(s, group, i, capacity).units;
+    return n;
+}
+
+// inclusive sum over the block's threads (whole warps)
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(~0u, v, o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sum[warp] = v;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) v += warp_sum[w];
+    return v;
+}
+
+// a block's part of the line, and the sequence that it stands in
+struct part_t {
+    int64_t total, begin, stop;
+    int blocks; // that have a part: none is empty
+    int group, heads;
+    int64_t capacity; // tokens that a row of the table can hold
+    int seq;
+    int64_t seq_begin, per_head;
+    seq_t s;
+};
+
+// where a unit lies
+struct place_t {
+    int head, tile;
+    item_t item;
+    int64_t item_begin;
+};
+
+// All threads of the block.  False: the block has no part.  `shared`: 34 words that nothing else uses meanwhile.
+template <int ROWS>
+__device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, part_t &l, int64_t *shared) {
+    const b200_kv_cache_t &c = p.cache;
+    const int tid = threadIdx.x, threads = blockDim.x;
+    int64_t *warp_sum = shared, *words = shared + 32;
+    l.group = (int)(p.q_heads / c.heads);
+    l.heads = (int)c.heads;
+    l.capacity = min((int64_t)0x7fffff00, c.table_cols * c.page);
+    l.total = 0;
+    for (int base = 0; base < c.seqs; base += threads) {
+        const int b = base + tid;
+        int64_t n = 0;
+        if (b < c.seqs) n = head_units<ROWS>(load_seq(c, b, p.rows), l.group, l.capacity) * l.heads;
+        n = block_scan(n, warp_sum);
+        if (tid == threads - 1) words[0] = n;
+        __syncthreads();
+        l.total += words[0];
+    }
+    l.blocks = (int)min((int64_t)gridDim.x, l.total);
+    if (blockIdx.x >= l.blocks) return false;
+    l.begin = l.total * blockIdx.x / l.blocks;
+    l.stop = l.total * (blockIdx.x + 1) / l.blocks;
+    // the sequence that the part begins in, and the units before it
+    l.seq = 0;
+    l.seq_begin = 0;
+    for (int base = 0; base < c.seqs; base += threads) {
+        const int b = base + tid;
+        int64_t n = 0;
+        if (b < c.seqs) n = head_units<ROWS>(load_seq(c, b, p.rows), l.group, l.capacity) * l.heads;
+        const int64_t upto = l.seq_begin + block_scan(n, warp_sum);
+        __syncthreads();
+        if (tid == 0) words[0] = -1;
+        __syncthreads();
+        if (upto > l.begin && upto - n <= l.begin) words[0] = b, words[1] = upto - n;
+        if (tid == threads - 1) warp_sum[0] = upto;
+        __syncthreads();
+        if (words[0] >= 0) {
+            l.seq = (int)words[0];
+            l.seq_begin = words[1];
+            break;
+        }
+        l.seq_begin = warp_sum[0];
+        __syncthreads();
+    }
+    l.s = load_seq(c, l.seq, p.rows);
+    l.per_head = head_units<ROWS>(l.s, l.group, l.capacity);
+    return true;
+}
+
+// the item at unit `at`, which never goes back
+template <int ROWS>
+__device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p, part_t &l, int64_t at) {
+    while (at - l.seq_begin >= l.per_head * l.heads) {
+        l.seq_begin += l.per_head * l.heads;
+        l.s = load_seq(p.cache, ++l.seq, p.rows);
+        l.per_head = head_units<ROWS>(l.s, l.group, l.capacity);
+    }
+    place_t q;
+    q.head = (int)((at - l.seq_begin) / l.per_head);
+    q.item_begin = l.seq_begin + q.head * l.per_head;
+    q.tile = 0;
+    q.item = item_of<ROWS>(l.s, l.group, 0, l.capacity);
+    while (at - q.item_begin >= q.item.units) {
+        q.item_begin += q.item.units;
+        q.item = item_of<ROWS>(l.s, l.group, ++q.tile, l.capacity);
+    }
+    return q;
+}
+
+// the block whose part holds unit u
+__device__ __forceinline__ int owner(const part_t &l, int64_t u) {
+    int64_t o = u * l.blocks / l.total;
+    while (l.total * (o + 1) / l.blocks <= u) ++o;
+    while (l.total * o / l.blocks > u) --o;
+    return (int)o;
+}
+
+// Scratch: a counter per block (parts done of the item that begins in its stretch of the line and ends in another's;
+// zero between launches), then per block two partial results: [0] of the item that it begins in, [1] of the one it ends in.
+__host__ __device__ inline size_t counter_bytes(int blocks) { return ((size_t)blocks * 4 + 255) / 256 * 256; }
+
+// the partial result of block b, one of those that share the item from `item_begin` on
+__device__ __forceinline__ size_t part_index(const part_t &l, int64_t item_begin, int first, int b) {
+    return (size_t)b * 2 + (b == first && l.total * b / l.blocks != item_begin ? 1 : 0);
+}
+
+} // namespace kv_line
+} // namespace b200

@@ -607,12 +607,18 @@ ATTEND = [  # lens, news, heads, group, page, dim, cache kind, q kind, before, b
     ([3000, 11], [130, 1], 2, 2, 32, 176, "e4m3", "bf16", 0, 1),
     ([61, 62], [1, 2], 2, 3, 7, 20, "s8", "f16", 0, 0),  # rows of 20 bytes
     ([90, 45], [40, 45], 3, 7, 13, 96, "s8", "bf16", 1, 0),
+    ([129], [129], 1, 1, 16, 128, "s8", "bf16", 0, 0),  # one row more than a tile of rows
+    ([128, 257], [128, 257], 1, 2, 64, 64, "e4m3", "bf16", 0, 0),
+    ([40, 1000], [3, 300], 2, 3, 48, 96, "s8", "f16", 0, 2),
+    ([900, 10, 0], [257, 20, 3], 1, 4, 128, 128, "e4m3", "f16", 2, 0),  # rows that see no token
+    ([5000], [64], 2, 1, 32, 128, "s8", "bf16", 0, 0),  # one item in many parts
+    ([2100, 2100], [700, 650], 3, 2, 16, 80, "s8", "bf16", 0, 0),
     ([50] * 70, [1] * 70, 1, 8, 16, 64, "s8", "bf16", 0, 0),
 ]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("impl", [None, "cuda:generic"])
+@pytest.mark.parametrize("impl", [None, "cuda:sm100:kv_attention_mma", "cuda:generic"])
 @pytest.mark.parametrize("lens,news,heads,group,page,dim,kind,src,before,behind", ATTEND)
 def test_attention(gpu, impl, lens, news, heads, group, page, dim, kind, src, before, behind):
     torch, types = _torch()
