@@ -43,12 +43,16 @@ struct smem_t {
     static constexpr int BYTES = (2 + 2 * STAGES) * MAT;
 };
 
-// scales of the tokens of a tile, 16 at a time; four tiles deep: the converters are at most two ahead of the slower softmax
+// The scales of a tile's tokens, 16 at a time, as the softmax takes them.  Four tiles deep: the converters are at most
+// two ahead of the slower softmax.
 struct scales_t {
-    float key[CHUNKS];      // below zero: no such page
-    float value_log[CHUNKS]; // log2
-    float value_inv[CHUNKS];
+    // x key scale, y 0 (-inf: no such page), z log2(value scale) - ref (-inf: no such page), w 2^-z
+    float4 chunk[CHUNKS];
+    float step; // what O is to be multiplied by: 2^(last tile's ref - this one's)
+    float up;   // 2^ref
 };
+
+constexpr float SMALL = 1.0842022e-19f; // 2^-63
 
 struct ctrl_t {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
@@ -108,7 +112,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
             "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
             : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_ld32_issue(uint32_t addr, uint32_t (&v)[32]) {
     asm volatile(
             "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
             "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -119,6 +123,9 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
             "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
             : "r"(addr)
             : "memory");
+}
+// all loads before it have arrived
+__device__ __forceinline__ void tmem_ld32_wait(uint32_t (&v)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
                  "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]),
@@ -126,6 +133,10 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
                  "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
                  :
                  : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
+    tmem_ld32_issue(addr, v);
+    tmem_ld32_wait(v);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
     asm volatile(
@@ -145,7 +156,27 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
             "r"(v[14]), "r"(v[15]), "r"(addr)
             : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+            : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+            "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+            : "r"(addr)
+            : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 
 // Shared-memory matrix descriptor, 128-byte swizzle: 128-byte rows, eight to an atom, atoms `stride` bytes apart along
 // the rows; `lead`: between blocks of 128-byte columns (used where the operand is N-major and wider than 64).
@@ -161,6 +192,32 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float lg2(float x) {
     float r;
     asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// two f32 at a time
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 // four codes -> two f16 pairs, exactly (s8: code + 128 in the low byte of 1024, minus 1152)
@@ -221,8 +278,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = ctrl->tmem_base;
-    // columns: S_0 | S_1 | O_0 | O_1
+    // Tensor memory columns: S_0 | S_1 | O_0 | O_1.  All 512 are this block's, so they begin at 0.
+    constexpr uint32_t tmem = 0;
     const int group = line.group;
 
     if (warp < SOFTMAX_WARPS) {
@@ -245,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             const int idx = q.tile * ROWS + t * TILE + r;
             const bool mine = t * TILE + r < rows;
             const int64_t at_row = s.begin + idx / group, at_head = (int64_t)q.head * group + idx % group;
-            float m = -INFINITY, l = 0.f, ref = -200.f;
+            float m = -INFINITY, l = 0.f, up = 0.f; // up: 2^ref
             if (active) {
                 // ---- the row's query: to f16 after a power of two that brings its largest element to [1, 2).
                 // A negative softmax scale turns the query round, so that factors of the scores are positive.
@@ -270,7 +327,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     const int e = top == 0 ? 127 : min(max((int)(top >> 23), 1), 253);
                     float down = __uint_as_float((uint32_t)(254 - e) << 23);
                     if (p.scale < 0.f) down = -down;
-                    factor = fabsf(p.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23);
+                    // this times a key scale, both held to 2^-63, stays a normal number: -inf times it is -inf
+                    factor = fmaxf(fabsf(p.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), SMALL);
                     uint8_t *to = smem_q + t * S::MAT;
 #pragma unroll
                     for (int i = 0; i < DP / 8; ++i) {
@@ -293,92 +351,100 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     s_phase ^= 1;
                     tc_fence_after();
                     const scales_t &sc = ctrl->scales[tile_i & 3];
-                    const bool masked = j * UNIT + UNIT - 1 > first_limit;
-                    const int seen = limit - j * UNIT; // columns 0 .. seen are seen
-                    // ---- the largest score, and the largest value scale
-                    float top = m, vtop = -300.f;
-                    bool gaps = false;
-#pragma unroll
-                    for (int h = 0; h < UNIT / 32; ++h) {
-                        uint32_t v[32];
-                        tmem_ld32(tmem_s + h * 32, v);
-                        if (masked) {
+                    uint32_t va[32], vb[32];
+                    if (j * UNIT + UNIT - 1 > first_limit) { // the last tiles: what a row does not see goes from its scores
+                        const int seen = limit - j * UNIT;   // columns 0 .. seen are seen
+#pragma unroll 1
+                        for (int h = 0; h < UNIT / 32; ++h) {
+                            tmem_ld32(tmem_s + h * 32, va);
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (h * 32 + i > seen) v[i] = 0xff800000u;
+                                if (h * 32 + i > seen) va[i] = 0xff800000u;
+                            tmem_st32(tmem_s + h * 32, va);
                         }
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float key = sc.key[h * 2 + k];
-                            gaps |= key < 0.f;
-                            vtop = fmaxf(vtop, sc.value_log[h * 2 + k]);
-                            float x = -INFINITY;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) x = fmaxf(x, __uint_as_float(v[k * 16 + i]));
-                            if (key >= 0.f) top = fmaxf(top, x * fmaxf(key * factor, 1.17549435e-38f));
-                        }
+                        tmem_wait_st();
                     }
-                    // ---- m and ref follow; O and the sum with them
-                    const float ref_now = vtop > ref ? ceilf(vtop) + 1.f : ref;
-                    const bool follow = top > m + 8.f; // also from -inf
-                    const float m_now = follow ? top : m;
-                    float fo = 1.f;
-                    if (follow || ref_now != ref) {
-                        const float d = follow ? ex2(m - m_now) : 1.f;
+                    tmem_ld32_issue(tmem_s, va);
+                    // O, the sum and the weights of this tile that are stored already (`done` columns) follow m and ref
+                    auto rescale = [&](float d, float fo, int done) {
+                        tmem_wait_st(); // what was stored is read here
                         l *= d;
-                        fo = d * ex2(ref - ref_now);
-                    }
-                    m = m_now;
-                    ref = ref_now;
-                    if (j > u0 && __any_sync(~0u, fo != 1.f)) {
+                        if (j > u0) {
+#pragma unroll 1
+                            for (int h = 0; h < DP / 16; ++h) {
+                                uint32_t v[16];
+                                tmem_ld16(tmem_o + h * 16, v);
 #pragma unroll
-                        for (int h = 0; h < DP / 32; ++h) {
-                            uint32_t v[32];
-                            tmem_ld32(tmem_o + h * 32, v);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * fo);
-                            tmem_st32(tmem_o + h * 32, v);
+                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * fo);
+                                tmem_st16(tmem_o + h * 16, v);
+                            }
                         }
-                    }
-                    // ---- weights
-                    const float base = (m == -INFINITY ? 0.f : m) + ref;
-                    const float ref_up = ex2(ref);
+#pragma unroll 1
+                        for (int h = 0; h < done; h += FINE ? 16 : 32) {
+                            uint32_t v[16];
+                            tmem_ld16(tmem_s + h, v);
+                            const uint32_t dd = pack_f16x2(d, d);
 #pragma unroll
-                    for (int h = 0; h < UNIT / 32; ++h) {
-                        uint32_t v[32], pw[16], rest[FINE ? 16 : 1];
-                        tmem_ld32(tmem_s + h * 32, v);
-                        if (masked) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (h * 32 + i > seen) v[i] = 0xff800000u;
+                            for (int i = 0; i < 16; ++i) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v[i]) : "r"(dd));
+                            tmem_st16(tmem_s + h, v);
                         }
+                    };
+                    up = sc.up;
+                    if (sc.step != 1.f && j > u0) { // the same for all rows
+                        tmem_ld32_wait(va);
+                        rescale(1.f, sc.step, 0);
+                    }
+                    // 32 columns: the largest score, m where that has outgrown it, the weights over the scores
+                    auto columns = [&](int h, uint32_t (&v)[32], uint32_t (&next)[32]) {
+                        tmem_ld32_wait(v);
+                        if (h + 1 < UNIT / 32) tmem_ld32_issue(tmem_s + (h + 1) * 32, next);
+                        const float4 c0 = sc.chunk[2 * h], c1 = sc.chunk[2 * h + 1];
+                        const float f0 = c0.x * factor, f1 = c1.x * factor;
+                        float x0 = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
+                        float x1 = max3(__uint_as_float(v[16]), __uint_as_float(v[17]), __uint_as_float(v[18]));
+#pragma unroll
+                        for (int i = 3; i < 15; i += 2) {
+                            x0 = max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                            x1 = max3(x1, __uint_as_float(v[16 + i]), __uint_as_float(v[17 + i]));
+                        }
+                        const float top = fmaxf(fmaf(fmaxf(x0, __uint_as_float(v[15])), f0, c0.y), fmaf(fmaxf(x1, __uint_as_float(v[31])), f1, c1.y));
+                        if (__any_sync(~0u, top > m + 8.f)) { // also from -inf
+                            const float m_now = top > m + 8.f ? top : m;
+                            const float d = m_now == m ? 1.f : ex2(m - m_now);
+                            if (h + 1 < UNIT / 32) tmem_ld32_wait(next);
+                            rescale(d, d, h * 32);
+                            m = m_now;
+                        }
+                        const float base = m == -INFINITY ? 0.f : m;
+                        uint32_t pw[16], rest[FINE ? 16 : 1];
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            const float key = sc.key[h * 2 + k];
-                            const float f = fmaxf(key * factor, 1.17549435e-38f);
-                            // scales below 2^-60 of the largest count as that: their values round to nothing, their weights stay in the sum
-                            const float vl = fmaxf(sc.value_log[h * 2 + k], ref - 60.f);
-                            const float off = gaps && key < 0.f ? -INFINITY : vl - base;
-                            const float back = fminf(sc.value_inv[h * 2 + k] * ref_up, 1.152921504606847e18f); // 2^60
-                            float sum = 0.f;
+                            const float off = (k ? c1.z : c0.z) - base;
+                            const uint64_t ff = f32x2(k ? f1 : f0, k ? f1 : f0), oo = f32x2(off, off);
+                            uint64_t sum = 0;
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
-                                const float x0 = ex2(fmaf(__uint_as_float(v[k * 16 + i]), f, off));
-                                const float x1 = ex2(fmaf(__uint_as_float(v[k * 16 + i + 1]), f, off));
-                                sum += x0;
-                                sum += x1;
-                                const uint32_t hi = pack_f16x2(x0, x1);
+                                const float2 x = unpack2(fma2(f32x2(__uint_as_float(v[k * 16 + i]), __uint_as_float(v[k * 16 + i + 1])), ff, oo));
+                                const float e0 = ex2(x.x), e1 = ex2(x.y);
+                                sum = add2(sum, f32x2(e0, e1));
+                                const uint32_t hi = pack_f16x2(e0, e1);
                                 pw[k * 8 + i / 2] = hi;
                                 if (FINE) {
                                     const float2 had = f16x2_to_f32(hi);
-                                    rest[FINE ? k * 8 + i / 2 : 0] = pack_f16x2(x0 - had.x, x1 - had.y);
+                                    rest[FINE ? k * 8 + i / 2 : 0] = pack_f16x2(e0 - had.x, e1 - had.y);
                                 }
                             }
-                            l = fmaf(sum, back, l);
+                            const float2 both = unpack2(sum);
+                            l = fmaf(both.x + both.y, k ? c1.w : c0.w, l);
                         }
-                        // over the 32 columns just read
+                        // over the columns just read; the first half, or both
                         tmem_st16(tmem_s + h * 32, pw);
                         if (FINE) tmem_st16(tmem_s + h * 32 + 16, rest);
+                    };
+#pragma unroll 1
+                    for (int h = 0; h < UNIT / 32; h += 2) {
+                        columns(h, va, vb);
+                        columns(h + 1, vb, va);
                     }
                     tmem_wait_st();
                     tc_fence_before();
@@ -394,7 +460,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
 
             // ---- the row's result, or its part of it
             const bool whole = u0 == 0 && u1 == q.item.units;
-            const float up = ref <= -200.f ? 0.f : ex2(ref);
             if (l != l) m = INFINITY; // a NaN among the scores, which no maximum shows
             char *to = (char *)p.dst + (at_row * p.dst_s0 + at_head * p.dst_s1) * 2;
             float *part = parts + (size_t)(blockIdx.x * 2 + (at == line.begin ? 0 : 1)) * part_size;
@@ -408,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             };
             if (active && ok) {
                 const float inv = l == 0.f ? 0.f : up / l;
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < DP / 32; ++h) {
                     uint32_t v[32];
                     tmem_ld32(tmem_o + h * 32, v);
@@ -483,10 +548,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         }
     } else if (warp < SOFTMAX_WARPS + CONVERT_WARPS) {
         // ---------------- codes to f16 ----------------
-        // Warp w has tokens 32 w .. of a tile: two runs of 16, each in one page.  CH lanes share a token (16 codes each), so an
-        // access of the warp covers 32 / CH tokens.
+        // Warp w has tokens 32 w .. of a tile: two runs of 16, each in one page.  An access of the warp covers 512 / DP tokens in
+        // groups of eight lanes: two tokens, 64 dims each, so that both the 64-byte reads and the stores (pieces
+        // 0, 2, 4, 6 of an even token, swizzled, and of the odd one next to it) use all that they touch.
         constexpr int CH = DP / 16, PER = 32 / CH, LOADS = 32 / PER;
-        const int w = warp - SOFTMAX_WARPS, cc = lane % CH, page = (int)c.page;
+        const int w = warp - SOFTMAX_WARPS, page = (int)c.page;
+        const int cc = DP == 64 ? lane & 3 : (lane & 3) + (lane >> 3 & 1) * 4; // 16 codes of a token
+        const int sub_row = DP == 64 ? lane >> 2 : (lane >> 4) * 2 + (lane >> 2 & 1);
         const bool takes = cc * 16 < c.dim;
         uint32_t tile_i = 0;
         int64_t at = line.begin;
@@ -500,146 +568,163 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             const int32_t *table = c.table + (int64_t)line.seq * c.table_s0;
             const uint8_t *keys = (const uint8_t *)c.key + q.head * c.s_head + cc * 16, *values = (const uint8_t *)c.value + q.head * c.s_head + cc * 16;
             uint4 kr[LOADS], vr[LOADS];
-            float ks[2], vs[2];
-            // where the two runs of tile j are; below zero: nowhere
-            auto find = [&](int j, int64_t (&place)[2], int (&page_at)[2]) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int tok = j * UNIT + w * 32 + h * 16;
-                    place[h] = -1;
-                    page_at[h] = 0;
-                    if (j < u1 && tok < end) {
-                        const int n = tok / page, slot = tok - n * page, phys = table[n];
-                        if (phys >= 0 && phys < c.pages) place[h] = (int64_t)phys * c.s_page + (int64_t)slot * c.s_slot, page_at[h] = phys;
-                        else flag_bad_page(c);
+            // every warp looks up all eight runs of a tile, one per lane, because `ref` needs all their scales
+            int64_t place = -1;
+            float ks = -1.f, vs = 0.f;
+            int n = (u0 * UNIT + lane * 16) / page, slot = u0 * UNIT + lane * 16 - n * page;
+            const int jump_n = UNIT / page, jump_slot = UNIT - jump_n * page;
+            auto find = [&](int j) {
+                place = -1, ks = -1.f, vs = 0.f;
+                if (lane < CHUNKS && j < u1 && j * UNIT + lane * 16 < end) {
+                    const int phys = table[n];
+                    if (phys >= 0 && phys < c.pages) {
+                        place = (int64_t)phys * c.s_page + (int64_t)slot * c.s_slot;
+                        const int64_t i = (int64_t)phys * c.heads + q.head;
+                        ks = c.key_scale[i], vs = c.value_scale[i];
+                    } else {
+                        flag_bad_page(c);
                     }
                 }
+                n += jump_n, slot += jump_slot;
+                if (slot >= page) slot -= page, ++n;
             };
-            auto load = [&](int j, const uint8_t *from, const int64_t (&place)[2], uint4 (&regs)[LOADS]) {
+            auto load = [&](int j, const uint8_t *from, uint4 (&regs)[LOADS]) {
+                const int64_t run[2] = {__shfl_sync(~0u, place, w * 2), __shfl_sync(~0u, place, w * 2 + 1)};
+                const int left = end - j * UNIT - w * 32;
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
-                    const int tok = i * PER + lane / CH, h = tok >> 4; // of the warp's 32
+                    const int tok = i * PER + sub_row; // of the warp's 32; the run is known at compile time
+                    const int64_t at_run = run[i * PER >> 4];
                     regs[i] = make_uint4(0, 0, 0, 0);
-                    const int64_t at_run = h ? place[1] : place[0];
-                    if (takes && at_run >= 0 && j * UNIT + w * 32 + tok < end)
-                        regs[i] = __ldg((const uint4 *)(from + at_run + (int64_t)(tok & 15) * c.s_slot));
-                }
-            };
-            auto load_scales = [&](const int64_t (&place)[2], const int (&page_at)[2]) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int64_t i = (int64_t)page_at[h] * c.heads + q.head;
-                    ks[h] = place[h] >= 0 ? c.key_scale[i] : -1.f;
-                    vs[h] = place[h] >= 0 ? c.value_scale[i] : 0.f;
+                    if (takes && at_run >= 0 && tok < left) regs[i] = __ldg((const uint4 *)(from + at_run + (tok & 15) * c.s_slot));
                 }
             };
             auto convert = [&](const uint4 (&regs)[LOADS], uint8_t *to) {
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
-                    const int row = w * 32 + i * PER + lane / CH;
+                    const int row = w * 32 + i * PER + sub_row;
                     const uint2 a = widen<S8>(regs[i].x), b = widen<S8>(regs[i].y), d = widen<S8>(regs[i].z), e = widen<S8>(regs[i].w);
-                    const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(d.x, d.y, e.x, e.y);
-                    // two 16-byte pieces; half of the lanes of a row store theirs the other way round: other banks
-                    const int swap = cc >> 2 & 1;
-                    *(uint4 *)(to + piece_at(row, cc * 2 + swap)) = swap ? hi : lo;
-                    *(uint4 *)(to + piece_at(row, cc * 2 + 1 - swap)) = swap ? lo : hi;
+                    *(uint4 *)(to + piece_at(row, cc * 2)) = make_uint4(a.x, a.y, b.x, b.y);
+                    *(uint4 *)(to + piece_at(row, cc * 2 + 1)) = make_uint4(d.x, d.y, e.x, e.y);
                 }
             };
-            int64_t place[2];
-            int page_at[2];
-            find(u0, place, page_at);
-            load_scales(place, page_at);
-            load(u0, keys, place, kr);
-            load(u0, values, place, vr);
+            float ref = -200.f;
+            find(u0);
+            load(u0, keys, kr);
+            load(u0, values, vr);
             for (int j = u0; j < u1; ++j, ++tile_i) {
                 const int st = tile_i % STAGES;
                 const uint32_t use = tile_i / STAGES;
                 // keys, and both scales: a softmax that sees the scores sees them
                 if (use > 0 && !(ok = warp_wait(&ctrl->k_empty[st], (use - 1) & 1, ctrl, status))) break;
-                if (lane < 2) {
-                    const float v = fmaxf(lane ? vs[1] : vs[0], 7.5231638e-37f); // 2^-120
-                    scales_t &sc = ctrl->scales[tile_i & 3];
-                    sc.key[w * 2 + lane] = lane ? ks[1] : ks[0];
-                    sc.value_log[w * 2 + lane] = lg2(v);
-                    sc.value_inv[w * 2 + lane] = 1.f / v;
+                {
+                    const float log = lg2(fmaxf(vs, 7.5231638e-37f)); // 2^-120 at least
+                    float top = lane < CHUNKS ? log : -200.f;
+#pragma unroll
+                    for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+                    top = __shfl_sync(~0u, top, 0);
+                    // with room, so that it seldom moves
+                    const float now = top > ref ? ceilf(top) + 1.f : ref;
+                    if (w == 0 && lane < CHUNKS) {
+                        scales_t &sc = ctrl->scales[tile_i & 3];
+                        const bool there = ks >= 0.f;
+                        // scales below 2^-60 of the largest count as that: their values round to nothing, their weights stay in the sum
+                        const float z = fmaxf(log - now, -60.f);
+                        sc.chunk[lane] = make_float4(fmaxf(ks, SMALL), there ? 0.f : -INFINITY, there ? z : -INFINITY, ex2(-z));
+                        if (lane == 0) sc.step = now == ref ? 1.f : ex2(ref - now), sc.up = ex2(now);
+                    }
+                    ref = now;
                 }
                 convert(kr, smem_k + st * S::MAT);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->k_full[st]);
-                find(j + 1, place, page_at);
-                load_scales(place, page_at);
-                load(j + 1, keys, place, kr);
+                find(j + 1);
+                load(j + 1, keys, kr);
                 if (use > 0 && !(ok = warp_wait(&ctrl->v_empty[st], (use - 1) & 1, ctrl, status))) break;
                 convert(vr, smem_v + st * S::MAT);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->v_full[st]);
-                load(j + 1, values, place, vr);
+                load(j + 1, values, vr);
             }
             at = q.item_begin + u1;
         }
-    } else if (lane == 0) {
+    } else {
         // ---------------- the MMAs ----------------
+        // The whole warp walks through the loops, so that descriptors and addresses are uniform values; one lane
+        // issues.  Tensor memory addresses are constants: the kernel allocates all columns.
         constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(TILE >> 4) << 24);
         constexpr uint32_t IDESC_S = IDESC | ((uint32_t)(UNIT >> 3) << 17);
         constexpr uint32_t IDESC_O = IDESC | (1u << 16) | ((uint32_t)(DP >> 3) << 17); // values are N-major
-        uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, tile_i = 0;
+        const uint64_t q_desc = make_desc(smem_u32(smem_q), 16, 1024), k_desc = make_desc(smem_u32(smem_k), 16, 1024);
+        const uint64_t v_desc = make_desc(smem_u32(smem_v), UNIT * 128, 1024);
+        uint32_t q_phase = 0, p_phase = 0, tile_i = 0; // a bit per tile
         int64_t at = line.begin;
         bool ok = true;
         auto scores = [&](int t, int st) { // S_t = Q_t K^T
-            const uint32_t a = smem_u32(smem_q + t * S::MAT), b = smem_u32(smem_k + st * S::MAT);
+            const uint64_t a = q_desc + (uint64_t)(t * (S::MAT >> 4)), b = k_desc + (uint64_t)(st * (S::MAT >> 4));
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t o = (uint32_t)((k >> 2) * (UNIT * 128) + (k & 3) * 32);
-                mma_ss(tmem + t * UNIT, make_desc(a + o, 16, 1024), make_desc(b + o, 16, 1024), IDESC_S, k != 0);
+                for (int k = 0; k < DP / 16; ++k) {
+                    const uint32_t o = (uint32_t)((k >> 2) * (UNIT * 128) + (k & 3) * 32) >> 4;
+                    mma_ss(t * UNIT, a + o, b + o, IDESC_S, k != 0);
+                }
+                tc_commit(&ctrl->s_full[t]);
             }
         };
-        auto weigh = [&](int t, int st, bool more) { // O_t += P_t V
-            const uint32_t b = smem_u32(smem_v + st * S::MAT);
+        auto weigh = [&](int t, int st, bool more, bool last) { // O_t += P_t V
+            const uint64_t b = v_desc + (uint64_t)(st * (S::MAT >> 4));
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < UNIT / 16; ++k) {
-                const uint64_t desc = make_desc(b + k * 2048, UNIT * 128, 1024);
-                const uint32_t a = tmem + t * UNIT + (k >> 1) * 32 + (k & 1) * 8;
-                mma_ts(tmem + 2 * UNIT + t * DP, a, desc, IDESC_O, more || k != 0);
-                if (FINE) mma_ts(tmem + 2 * UNIT + t * DP, a + 16, desc, IDESC_O, 1);
+                for (int k = 0; k < UNIT / 16; ++k) {
+                    const uint32_t a = t * UNIT + (k >> 1) * 32 + (k & 1) * 8;
+                    mma_ts(2 * UNIT + t * DP, a, b + k * (2048 >> 4), IDESC_O, more || k != 0);
+                    if (FINE) mma_ts(2 * UNIT + t * DP, a + 16, b + k * (2048 >> 4), IDESC_O, 1);
+                }
+                if (last) tc_commit(&ctrl->o_full[t]);
             }
+        };
+        auto commit = [&](uint64_t *bar) {
+            if (elect_one()) tc_commit(bar);
         };
         while (at < line.stop && ok) {
             const place_t q = find_item<ROWS>(p, line, at);
             const seq_t s = line.s;
             const int u0 = (int)(at - q.item_begin), u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
-            const int rows = (s.end - s.begin) * group - q.tile * ROWS;
-            const int tiles = rows > TILE ? 2 : 1, n = u1 - u0;
-            if (!(ok = mbar_wait(&ctrl->k_full[tile_i % STAGES], (tile_i / STAGES) & 1, ctrl, status))) break;
-            for (int t = 0; t < tiles && ok; ++t) {
-                if (!(ok = mbar_wait(&ctrl->q_full[t], q_phase[t], ctrl, status))) break;
-                q_phase[t] ^= 1;
+            const int rows = (s.end - s.begin) * group - q.tile * ROWS, n = u1 - u0;
+            const bool two = rows > TILE;
+            if (!(ok = warp_wait(&ctrl->k_full[tile_i % STAGES], (tile_i / STAGES) & 1, ctrl, status))) break;
+            if (!(ok = warp_wait(&ctrl->q_full[0], q_phase & 1, ctrl, status))) break;
+            q_phase ^= 1;
+            tc_fence_after();
+            scores(0, tile_i % STAGES);
+            if (two) {
+                if (!(ok = warp_wait(&ctrl->q_full[1], q_phase >> 1, ctrl, status))) break;
+                q_phase ^= 2;
                 tc_fence_after();
-                scores(t, tile_i % STAGES);
-                tc_commit(&ctrl->s_full[t]);
+                scores(1, tile_i % STAGES);
             }
-            if (!ok) break;
-            tc_commit(&ctrl->k_empty[tile_i % STAGES]);
-            for (int j = 0; j < n && ok; ++j, ++tile_i) {
+            commit(&ctrl->k_empty[tile_i % STAGES]);
+            for (int j = 0; j < n; ++j, ++tile_i) {
                 const int st = tile_i % STAGES, next = (tile_i + 1) % STAGES;
-                if (!(ok = mbar_wait(&ctrl->v_full[st], (tile_i / STAGES) & 1, ctrl, status))) break;
-                if (j + 1 < n && !(ok = mbar_wait(&ctrl->k_full[next], ((tile_i + 1) / STAGES) & 1, ctrl, status))) break;
-                for (int t = 0; t < tiles; ++t) {
-                    if (!(ok = mbar_wait(&ctrl->p_full[t], p_phase[t], ctrl, status))) break;
-                    p_phase[t] ^= 1;
+                const bool last = j + 1 == n;
+                if (!(ok = warp_wait(&ctrl->v_full[st], (tile_i / STAGES) & 1, ctrl, status))) break;
+                if (!last && !(ok = warp_wait(&ctrl->k_full[next], ((tile_i + 1) / STAGES) & 1, ctrl, status))) break;
+                if (!(ok = warp_wait(&ctrl->p_full[0], p_phase & 1, ctrl, status))) break;
+                p_phase ^= 1;
+                tc_fence_after();
+                weigh(0, st, j > 0, last);
+                if (!last) scores(0, next);
+                if (two) {
+                    if (!(ok = warp_wait(&ctrl->p_full[1], p_phase >> 1, ctrl, status))) break;
+                    p_phase ^= 2;
                     tc_fence_after();
-                    weigh(t, st, j > 0);
-                    if (j + 1 < n) {
-                        scores(t, next);
-                        tc_commit(&ctrl->s_full[t]);
-                    } else {
-                        tc_commit(&ctrl->o_full[t]);
-                    }
+                    weigh(1, st, j > 0, last);
+                    if (!last) scores(1, next);
                 }
-                if (!ok) break;
-                tc_commit(&ctrl->v_empty[st]);
-                if (j + 1 < n) tc_commit(&ctrl->k_empty[next]);
+                commit(&ctrl->v_empty[st]);
+                if (!last) commit(&ctrl->k_empty[next]);
             }
             at = q.item_begin + u1;
         }
