@@ -10,7 +10,7 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row, so maximum and sum need no exchange; queries
 //                    on the way in, results on the way out
 //   warps 8-11       codes from the pages to f16 tiles in shared memory (exact), a tile ahead in registers
-//   warp 12          one thread issues all MMAs: QK_0(j+1) behind PV_0(j), QK_1(j+1) behind PV_1(j), so that one
+//   warp 12          (of four; the others hand in their registers) one thread issues all MMAs: QK_0(j+1) behind PV_0(j), QK_1(j+1) behind PV_1(j), so that one
 //                    tile's softmax runs beside the other's products
 //
 // The two scales stay out of the products.  A page holds a multiple of 16 tokens here, so 16 neighbouring tokens share
@@ -30,7 +30,10 @@ namespace {
 using namespace kv_line;
 
 constexpr int TILE = 128, ROWS = 2 * TILE; // query rows of a tile and of an item
-constexpr int SOFTMAX_WARPS = 8, CONVERT_WARPS = 4, WARPS = SOFTMAX_WARPS + CONVERT_WARPS + 1, THREADS = WARPS * 32;
+constexpr int SOFTMAX_WARPS = 8, CONVERT_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + CONVERT_WARPS, WARPS = MMA_WARP + 4, THREADS = WARPS * 32;
+// registers per thread: what the launch gives every warp, and how the four groups of four warps share it
+constexpr int REGS = 128, SOFTMAX_REGS = 176, CONVERT_REGS = 104, MMA_REGS = 56;
+static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * REGS && THREADS * REGS <= 65536, "");
 constexpr int STAGES = 2;  // of keys and of values
 constexpr int CHUNKS = UNIT / 16;
 constexpr uint32_t TMEM_COLS = 512;
@@ -75,10 +78,10 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+            : "r"(smem_u32(bar)), "r"(parity)
             : "memory");
     return ok != 0;
 }
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == WARPS - 1) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctrl->tmem_base)), "r"(TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -283,6 +286,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     const int group = line.group;
 
     if (warp < SOFTMAX_WARPS) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
         // ---------------- softmax: row r of tile t ----------------
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -293,9 +297,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         uint32_t s_phase = 0, o_phase = 0, tile_i = 0; // tile_i: tiles of tokens since the launch
         int64_t at = line.begin;
         bool ok = true; // once a wait has run out, only the barriers among the softmax warps are kept up
+        place_t q = find_item<ROWS>(p, line, at);
+        seq_t s = line.s;
+        // this thread's query row of an item, as it is, into its place in shared memory
+        auto fetch = [&](const place_t &item, const seq_t &seq) {
+            const int idx = item.tile * ROWS + t * TILE + r;
+            if (idx < (seq.end - seq.begin) * group) {
+                const char *from = (const char *)p.query
+                        + ((int64_t)(seq.begin + idx / group) * p.query_s0 + ((int64_t)item.head * group + idx % group) * p.query_s1) * 2;
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i)
+                    if (i * 8 < c.dim)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_q + t * S::MAT + piece_at(r, i))), "l"(from + i * 16)
+                                     : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch(q, s);
         while (at < line.stop) {
-            const place_t q = find_item<ROWS>(p, line, at);
-            const seq_t s = line.s;
             const int u0 = (int)(at - q.item_begin), u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
             const int rows = (s.end - s.begin) * group - q.tile * ROWS; // that exist from here on
             const bool active = ok && rows > t * TILE;
@@ -303,6 +322,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             const bool mine = t * TILE + r < rows;
             const int64_t at_row = s.begin + idx / group, at_head = (int64_t)q.head * group + idx % group;
             float m = -INFINITY, l = 0.f, up = 0.f; // up: 2^ref
+            const int64_t at_next = q.item_begin + u1;
+            place_t q_next = q;
+            seq_t s_next = s;
+            auto fetch_next = [&]() { // once the scores of the item's last tile are there, its queries are not needed any more
+                if (at_next < line.stop) {
+                    q_next = find_item<ROWS>(p, line, at_next);
+                    s_next = line.s;
+                    fetch(q_next, s_next);
+                }
+            };
             if (active) {
                 // ---- the row's query: to f16 after a power of two that brings its largest element to [1, 2).
                 // A negative softmax scale turns the query round, so that factors of the scores are positive.
@@ -310,14 +339,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 const int first_limit = __shfl_sync(~0u, limit, 0); // the smallest of the warp's rows that exist
                 float factor;
                 {
-                    uint4 w[DP / 8];
+                    uint8_t *to = smem_q + t * S::MAT;
                     uint32_t top = 0;
-                    const char *from = (const char *)p.query + (at_row * p.query_s0 + at_head * p.query_s1) * 2;
-#pragma unroll
-                    for (int i = 0; i < DP / 8; ++i) w[i] = mine && i * 8 < c.dim ? *(const uint4 *)(from + i * 16) : make_uint4(0, 0, 0, 0);
-#pragma unroll
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 4
                     for (int i = 0; i < DP / 8; ++i) {
-                        const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (mine && i * 8 < c.dim) w = *(const uint4 *)(to + piece_at(r, i));
+                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
                             const float2 f = bf16 ? bf16x2_to_f32(x[h]) : f16x2_to_f32(x[h]);
@@ -329,10 +358,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     if (p.scale < 0.f) down = -down;
                     // this times a key scale, both held to 2^-63, stays a normal number: -inf times it is -inf
                     factor = fmaxf(fabsf(p.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), SMALL);
-                    uint8_t *to = smem_q + t * S::MAT;
-#pragma unroll
+#pragma unroll 4
                     for (int i = 0; i < DP / 8; ++i) {
-                        const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (mine && i * 8 < c.dim) w = *(const uint4 *)(to + piece_at(r, i));
+                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
                         uint32_t y[4];
 #pragma unroll
                         for (int h = 0; h < 4; ++h) {
@@ -350,6 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     if (!(ok = warp_wait(&ctrl->s_full[t], s_phase, ctrl, status))) break;
                     s_phase ^= 1;
                     tc_fence_after();
+                    if (j + 1 == u1) fetch_next();
                     const scales_t &sc = ctrl->scales[tile_i & 3];
                     uint32_t va[32], vb[32];
                     if (j * UNIT + UNIT - 1 > first_limit) { // the last tiles: what a row does not see goes from its scores
@@ -456,6 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 tc_fence_after();
             } else {
                 tile_i += (uint32_t)(u1 - u0);
+                fetch_next();
             }
 
             // ---- the row's result, or its part of it
@@ -544,9 +576,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     }
                 }
             }
-            at = q.item_begin + u1;
+            at = at_next;
+            q = q_next;
+            s = s_next;
         }
-    } else if (warp < SOFTMAX_WARPS + CONVERT_WARPS) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else if (warp < MMA_WARP) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
         // ---------------- codes to f16 ----------------
         // Warp w has tokens 32 w .. of a tile: two runs of 16, each in one page.  An access of the warp covers 512 / DP tokens in
         // groups of eight lanes: two tokens, 64 dims each, so that both the 64-byte reads and the stores (pieces
@@ -556,6 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         const int cc = DP == 64 ? lane & 3 : (lane & 3) + (lane >> 3 & 1) * 4; // 16 codes of a token
         const int sub_row = DP == 64 ? lane >> 2 : (lane >> 4) * 2 + (lane >> 2 & 1);
         const bool takes = cc * 16 < c.dim;
+        const int64_t lane_at = sub_row * c.s_slot, per_step = PER * c.s_slot;
         uint32_t tile_i = 0;
         int64_t at = line.begin;
         bool ok = true;
@@ -591,12 +628,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             auto load = [&](int j, const uint8_t *from, uint4 (&regs)[LOADS]) {
                 const int64_t run[2] = {__shfl_sync(~0u, place, w * 2), __shfl_sync(~0u, place, w * 2 + 1)};
                 const int left = end - j * UNIT - w * 32;
+                if (DP == c.dim && (run[0] | run[1]) >= 0 && left >= 32) { // all there
+                    const uint8_t *at_run[2] = {from + run[0] + lane_at, from + run[1] + lane_at};
+#pragma unroll
+                    for (int i = 0; i < LOADS; ++i) // a run's accesses are PER tokens apart
+                        regs[i] = __ldg((const uint4 *)(at_run[i * PER >> 4] + (i % (16 / PER)) * per_step));
+                    return;
+                }
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
                     const int tok = i * PER + sub_row; // of the warp's 32; the run is known at compile time
-                    const int64_t at_run = run[i * PER >> 4];
                     regs[i] = make_uint4(0, 0, 0, 0);
-                    if (takes && at_run >= 0 && tok < left) regs[i] = __ldg((const uint4 *)(from + at_run + (tok & 15) * c.s_slot));
+                    if (takes && run[i * PER >> 4] >= 0 && tok < left)
+                        regs[i] = __ldg((const uint4 *)(from + run[i * PER >> 4] + (tok & 15) * c.s_slot));
                 }
             };
             auto convert = [&](const uint4 (&regs)[LOADS], uint8_t *to) {
@@ -651,6 +695,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             at = q.item_begin + u1;
         }
     } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MMA_REGS));
         // ---------------- the MMAs ----------------
         // The whole warp walks through the loops, so that descriptors and addresses are uniform values; one lane
         // issues.  Tensor memory addresses are constants: the kernel allocates all columns.
@@ -688,7 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         auto commit = [&](uint64_t *bar) {
             if (elect_one()) tc_commit(bar);
         };
-        while (at < line.stop && ok) {
+        while (warp == MMA_WARP && at < line.stop && ok) {
             const place_t q = find_item<ROWS>(p, line, at);
             const seq_t s = line.s;
             const int u0 = (int)(at - q.item_begin), u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
@@ -731,7 +776,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     }
     // all roles are through (the MMAs too: every one was waited for by way of o_full, unless a wait ran out)
     __syncthreads();
-    if (warp == WARPS - 1) {
+    if (warp == MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }

@@ -18,23 +18,46 @@ struct item_t {
     int units;  // one at least: rows that see nothing are still written
 };
 
+// The items of one key head of a sequence, in order; without a division per item.
 template <int ROWS>
-__device__ __forceinline__ item_t item_of(const seq_t &s, int group, int tile, int64_t capacity) {
-    const int rows = (s.end - s.begin) * group;
-    const int last = (min((tile + 1) * ROWS, rows) - 1) / group; // its newest token
-    const int64_t t = max(0, s.first + last + 1);
-    item_t i;
-    i.tokens = (int)min(t, capacity);
-    i.units = max(1, (i.tokens + UNIT - 1) / UNIT);
-    return i;
-}
+struct items_t {
+    int rows, tokens, group, first, tile = 0;
+    int last, rest;       // ((tile + 1) * ROWS - 1) / group and what is left
+    int step, step_rest;  // ROWS / group and what is left
+    int64_t capacity;
+
+    __device__ __forceinline__ items_t(const seq_t &s, int group_, int64_t capacity_) {
+        group = group_;
+        capacity = capacity_;
+        first = s.first;
+        tokens = s.end - s.begin;
+        rows = tokens * group;
+        step = ROWS / group;
+        step_rest = ROWS - step * group;
+        last = (ROWS - 1) / group;
+        rest = ROWS - 1 - last * group;
+    }
+    __device__ __forceinline__ bool there() const { return tile * ROWS < rows; }
+    __device__ __forceinline__ item_t get() const {
+        const int newest = min(last, tokens - 1); // token of its last row
+        item_t i;
+        i.tokens = (int)min((int64_t)max(0, first + newest + 1), capacity);
+        i.units = max(1, (i.tokens + UNIT - 1) / UNIT);
+        return i;
+    }
+    __device__ __forceinline__ void next() {
+        ++tile;
+        last += step;
+        rest += step_rest;
+        if (rest >= group) rest -= group, ++last;
+    }
+};
 
 // units of one key head of a sequence
 template <int ROWS>
 __device__ __forceinline__ int64_t head_units(const seq_t &s, int group, int64_t capacity) {
     int64_t n = 0;
-    const int tiles = ((s.end - s.begin) * group + ROWS - 1) / ROWS;
-    for (int i = 0; i < tiles; ++i) n += item_of<ROWS>(s, group, i, capacity).units;
+    for (items_t<ROWS> i(s, group, capacity); i.there(); i.next()) n += i.get().units;
     return n;
 }
 
@@ -132,12 +155,14 @@ __device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p
     place_t q;
     q.head = (int)((at - l.seq_begin) / l.per_head);
     q.item_begin = l.seq_begin + q.head * l.per_head;
-    q.tile = 0;
-    q.item = item_of<ROWS>(l.s, l.group, 0, l.capacity);
+    items_t<ROWS> i(l.s, l.group, l.capacity);
+    q.item = i.get();
     while (at - q.item_begin >= q.item.units) {
         q.item_begin += q.item.units;
-        q.item = item_of<ROWS>(l.s, l.group, ++q.tile, l.capacity);
+        i.next();
+        q.item = i.get();
     }
+    q.tile = i.tile;
     return q;
 }
 
