@@ -10,7 +10,8 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row, so maximum and sum need no exchange; queries
 //                    on the way in, results on the way out
 //   warps 8-11       codes from the pages to f16 tiles in shared memory (exact), a tile ahead in registers
-//   warp 12          (of four; the others hand in their registers) one thread issues all MMAs: QK_0(j+1) behind PV_0(j), QK_1(j+1) behind PV_1(j), so that one
+//   warp 13          finds the block's items ahead of all others and lays them out in shared memory
+//   warp 12          one thread issues all MMAs: QK_0(j+1) behind PV_0(j), QK_1(j+1) behind PV_1(j), so that one
 //                    tile's softmax runs beside the other's products
 //
 // The two scales stay out of the products.  A page holds a multiple of 16 tokens here, so 16 neighbouring tokens share
@@ -57,8 +58,25 @@ struct scales_t {
 
 constexpr float SMALL = 1.0842022e-19f; // 2^-63
 
+// a stretch of an item's tokens: what one block does of it
+struct segment_t {
+    int begin, rows;   // of the sequence, in the batch; query rows (x group) that exist from the item's first on, 0: no more segments
+    int row0, first;   // the item's first query row in the sequence; token of the sequence's first row
+    int head, seq;
+    int tokens;        // that the item's last row sees
+    int u0, u1;        // units, of
+    int units;
+    int c0, c1;        // the blocks that share the item
+    int slot;          // where its partial result goes
+    int parity;        // which of block c0's two partial results is the item's
+    int over;          // whether the sequence has tokens beyond the table
+};
+constexpr int SEGMENTS = 4;
+
 struct ctrl_t {
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+    uint64_t seg_full[SEGMENTS], seg_empty[SEGMENTS];
+    segment_t segments[SEGMENTS];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], join;
     uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
     uint32_t tmem_base;
     volatile uint32_t abort;
@@ -269,6 +287,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             mbar_init(&ctrl->k_empty[i], 1);
             mbar_init(&ctrl->v_empty[i], 1);
         }
+        for (int i = 0; i < SEGMENTS; ++i) {
+            mbar_init(&ctrl->seg_full[i], 1);
+            mbar_init(&ctrl->seg_empty[i], SOFTMAX_WARPS + CONVERT_WARPS + 1);
+        }
+        mbar_init(&ctrl->join, SOFTMAX_WARPS);
         ctrl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -284,6 +307,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     // Tensor memory columns: S_0 | S_1 | O_0 | O_1.  All 512 are this block's, so they begin at 0.
     constexpr uint32_t tmem = 0;
     const int group = line.group;
+    // the segment of number i, once it is laid out (nullptr when a wait ran out); given back by every warp that took it
+    auto take = [&](uint32_t i) -> const segment_t * {
+        return warp_wait(&ctrl->seg_full[i % SEGMENTS], (i / SEGMENTS) & 1, ctrl, status) ? &ctrl->segments[i % SEGMENTS] : nullptr;
+    };
+    auto give_back = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctrl->seg_empty[i % SEGMENTS]);
+    };
 
     if (warp < SOFTMAX_WARPS) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
@@ -295,16 +326,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         float *parts = (float *)((char *)p.scratch + counter_bytes(gridDim.x));
         constexpr size_t part_size = (size_t)ROWS * (DP + 2);
         uint32_t s_phase = 0, o_phase = 0, tile_i = 0; // tile_i: tiles of tokens since the launch
-        int64_t at = line.begin;
-        bool ok = true; // once a wait has run out, only the barriers among the softmax warps are kept up
-        place_t q = find_item<ROWS>(p, line, at);
-        seq_t s = line.s;
-        // this thread's query row of an item, as it is, into its place in shared memory
-        auto fetch = [&](const place_t &item, const seq_t &seq) {
-            const int idx = item.tile * ROWS + t * TILE + r;
-            if (idx < (seq.end - seq.begin) * group) {
+        bool ok = true;
+        uint32_t join_phase = 0;
+        auto join = [&]() { // all softmax warps
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctrl->join);
+            ok = warp_wait(&ctrl->join, join_phase, ctrl, status);
+            join_phase ^= 1;
+            return ok;
+        };
+        // this thread's query row of a segment, as it is, into its place in shared memory
+        auto fetch = [&](const segment_t &g) {
+            if (t * TILE + r < g.rows) {
+                const int idx = g.row0 + t * TILE + r;
                 const char *from = (const char *)p.query
-                        + ((int64_t)(seq.begin + idx / group) * p.query_s0 + ((int64_t)item.head * group + idx % group) * p.query_s1) * 2;
+                        + ((int64_t)(g.begin + idx / group) * p.query_s0 + ((int64_t)g.head * group + idx % group) * p.query_s1) * 2;
 #pragma unroll
                 for (int i = 0; i < DP / 8; ++i)
                     if (i * 8 < c.dim)
@@ -313,69 +349,66 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        fetch(q, s);
-        while (at < line.stop) {
-            const int u0 = (int)(at - q.item_begin), u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
-            const int rows = (s.end - s.begin) * group - q.tile * ROWS; // that exist from here on
-            const bool active = ok && rows > t * TILE;
-            const int idx = q.tile * ROWS + t * TILE + r;
-            const bool mine = t * TILE + r < rows;
-            const int64_t at_row = s.begin + idx / group, at_head = (int64_t)q.head * group + idx % group;
-            float m = -INFINITY, l = 0.f, up = 0.f; // up: 2^ref
-            const int64_t at_next = q.item_begin + u1;
-            place_t q_next = q;
-            seq_t s_next = s;
-            auto fetch_next = [&]() { // once the scores of the item's last tile are there, its queries are not needed any more
-                if (at_next < line.stop) {
-                    q_next = find_item<ROWS>(p, line, at_next);
-                    s_next = line.s;
-                    fetch(q_next, s_next);
+        // The row of an item that `fetch` brought: to f16 after a power of two that brings its largest element to [1, 2).
+        // A negative softmax scale turns the query round, so that factors of the scores are positive.
+        auto prepare = [&](bool there) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            uint8_t *to = smem_q + t * S::MAT;
+            uint32_t top2 = 0; // the largest magnitudes' bits, of even and of odd elements
+#pragma unroll 4
+            for (int i = 0; i < DP / 8; ++i) {
+                if (!there || i * 8 >= c.dim) *(uint4 *)(to + piece_at(r, i)) = make_uint4(0, 0, 0, 0);
+                const uint4 w = *(const uint4 *)(to + piece_at(r, i));
+                top2 = __vmaxu2(__vmaxu2(top2, w.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(w.y & 0x7fff7fffu, w.z & 0x7fff7fffu), w.w & 0x7fff7fffu));
+            }
+            const float2 tops = bf16 ? bf16x2_to_f32(top2) : f16x2_to_f32(top2);
+            const uint32_t top = max(__float_as_uint(tops.x), __float_as_uint(tops.y));
+            const int e = top == 0 ? 127 : min(max((int)(top >> 23), 1), 253);
+            float down = __uint_as_float((uint32_t)(254 - e) << 23);
+            if (p.scale < 0.f) down = -down;
+#pragma unroll 4
+            for (int i = 0; i < DP / 8; ++i) {
+                const uint4 w = *(const uint4 *)(to + piece_at(r, i));
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                uint32_t y[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const float2 f = bf16 ? bf16x2_to_f32(x[h]) : f16x2_to_f32(x[h]);
+                    y[h] = pack_f16x2(f.x * down, f.y * down);
                 }
+                *(uint4 *)(to + piece_at(r, i)) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctrl->q_full[t]);
+            // the factor of the row's scores, in log2.  It times a key scale, both held to 2^-63, stays a normal number: -inf times
+            // it is -inf
+            return fmaxf(fabsf(p.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), SMALL);
+        };
+        float factor = 0.f;
+        uint32_t seg_i = 0;
+        const segment_t *seg = take(0);
+        if (seg) {
+            fetch(*seg);
+            if (seg->rows > t * TILE) factor = prepare(t * TILE + r < seg->rows);
+        }
+        while (seg && seg->rows > 0) {
+            const int u0 = seg->u0, u1 = seg->u1;
+            const bool active = ok && seg->rows > t * TILE, mine = t * TILE + r < seg->rows;
+            float m = -INFINITY, l = 0.f, up = 0.f; // up: 2^ref
+            // the next segment: its queries come while this one's last tile is worked on, once that one's scores are there
+            const segment_t *next = nullptr;
+            float factor_next = 0.f;
+            auto fetch_next = [&]() {
+                next = take(seg_i + 1);
+                if (next) fetch(*next);
+            };
+            auto prepare_next = [&]() {
+                if (next && next->rows > t * TILE) factor_next = prepare(t * TILE + r < next->rows);
             };
             if (active) {
-                // ---- the row's query: to f16 after a power of two that brings its largest element to [1, 2).
-                // A negative softmax scale turns the query round, so that factors of the scores are positive.
-                const int limit = mine ? s.first + idx / group : -1;
+                const int limit = mine ? seg->first + (seg->row0 + t * TILE + r) / group : -1;
                 const int first_limit = __shfl_sync(~0u, limit, 0); // the smallest of the warp's rows that exist
-                float factor;
-                {
-                    uint8_t *to = smem_q + t * S::MAT;
-                    uint32_t top = 0;
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll 4
-                    for (int i = 0; i < DP / 8; ++i) {
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (mine && i * 8 < c.dim) w = *(const uint4 *)(to + piece_at(r, i));
-                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const float2 f = bf16 ? bf16x2_to_f32(x[h]) : f16x2_to_f32(x[h]);
-                            top = max(top, max(__float_as_uint(fabsf(f.x)), __float_as_uint(fabsf(f.y))));
-                        }
-                    }
-                    const int e = top == 0 ? 127 : min(max((int)(top >> 23), 1), 253);
-                    float down = __uint_as_float((uint32_t)(254 - e) << 23);
-                    if (p.scale < 0.f) down = -down;
-                    // this times a key scale, both held to 2^-63, stays a normal number: -inf times it is -inf
-                    factor = fmaxf(fabsf(p.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)e << 23), SMALL);
-#pragma unroll 4
-                    for (int i = 0; i < DP / 8; ++i) {
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (mine && i * 8 < c.dim) w = *(const uint4 *)(to + piece_at(r, i));
-                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-                        uint32_t y[4];
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const float2 f = bf16 ? bf16x2_to_f32(x[h]) : f16x2_to_f32(x[h]);
-                            y[h] = pack_f16x2(f.x * down, f.y * down);
-                        }
-                        *(uint4 *)(to + piece_at(r, i)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctrl->q_full[t]);
-
                 for (int j = u0; j < u1; ++j, ++tile_i) {
                     if (!(ok = warp_wait(&ctrl->s_full[t], s_phase, ctrl, status))) break;
                     s_phase ^= 1;
@@ -482,19 +515,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctrl->p_full[t]);
                 }
-                if (ok) ok = warp_wait(&ctrl->o_full[t], o_phase, ctrl, status);
+                if (ok) {
+                    prepare_next(); // beside the last products
+                    ok = warp_wait(&ctrl->o_full[t], o_phase, ctrl, status);
+                }
                 o_phase ^= 1;
                 tc_fence_after();
             } else {
                 tile_i += (uint32_t)(u1 - u0);
                 fetch_next();
+                prepare_next();
             }
 
             // ---- the row's result, or its part of it
-            const bool whole = u0 == 0 && u1 == q.item.units;
+            const bool whole = u0 == 0 && u1 == seg->units;
             if (l != l) m = INFINITY; // a NaN among the scores, which no maximum shows
-            char *to = (char *)p.dst + (at_row * p.dst_s0 + at_head * p.dst_s1) * 2;
-            float *part = parts + (size_t)(blockIdx.x * 2 + (at == line.begin ? 0 : 1)) * part_size;
+            const int idx = seg->row0 + t * TILE + r;
+            char *to = (char *)p.dst + ((int64_t)(seg->begin + idx / group) * p.dst_s0 + ((int64_t)seg->head * group + idx % group) * p.dst_s1) * 2;
+            float *part = parts + (size_t)(blockIdx.x * 2 + seg->slot) * part_size;
             const int pr = t * TILE + r; // row of the item
             auto put = [&](int d, const float (&x)[8], float inv) { // eight dims of the result
                 if (d >= c.dim) return;
@@ -527,58 +565,57 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 tc_fence_before(); // O may be written again after the next arrival
                 if (!whole && mine) part[pr] = m, part[ROWS + pr] = l;
             }
-            if (!whole) {
+            if (!whole && ok) {
                 // an item in several parts: the last block to finish one puts them together, in the order of the parts
-                const int c0 = owner(line, q.item_begin), c1 = owner(line, q.item_begin + q.item.units - 1);
+                const int c0 = seg->c0, c1 = seg->c1;
                 __threadfence();
-                asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_WARPS * 32) : "memory");
-                if (threadIdx.x == 0) {
+                if (join() && threadIdx.x == 0) {
                     uint32_t *count = (uint32_t *)p.scratch + c0;
                     const bool is_last = atomicAdd(count, 1u) == (uint32_t)(c1 - c0);
                     if (is_last) *count = 0; // as it was found
                     ctrl->last_part = is_last;
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_WARPS * 32) : "memory");
-                const bool is_last = ctrl->last_part;
-                asm volatile("bar.sync 1, %0;" ::"n"(SOFTMAX_WARPS * 32) : "memory"); // read before it is set again
-                if (is_last && mine) {
+                if (ok && join() && ctrl->last_part && mine) {
                     __threadfence();
-                    auto part_of = [&](int b) { return parts + part_index(line, q.item_begin, c0, b) * part_size; };
+                    auto part_of = [&](int b) { return parts + ((size_t)b * 2 + (b == c0 ? seg->parity : 0)) * part_size; };
                     float mm = -INFINITY, ll = 0.f;
+#pragma unroll 4
                     for (int b = c0; b <= c1; ++b) mm = fmaxf(mm, __ldcg(part_of(b) + pr));
+#pragma unroll 4
                     for (int b = c0; b <= c1; ++b) {
-                        const float mb = __ldcg(part_of(b) + pr), f = mb == -INFINITY ? 0.f : ex2(mb - mm);
-                        if (f != 0.f) ll = fmaf(__ldcg(part_of(b) + ROWS + pr), f, ll);
+                        const float mb = __ldcg(part_of(b) + pr), lb = __ldcg(part_of(b) + ROWS + pr), f = mb == -INFINITY ? 0.f : ex2(mb - mm);
+                        if (f != 0.f) ll = fmaf(lb, f, ll);
                     }
                     const float inv = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll 1
-                    for (int d = 0; d < DP; d += 32) {
-                        float x[4][8];
+                    for (int d = 0; d < DP; d += 64) {
+                        float x[8][8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 8; ++i)
 #pragma unroll
                             for (int k = 0; k < 8; ++k) x[i][k] = 0.f;
+#pragma unroll 1
                         for (int b = c0; b <= c1; ++b) {
+                            const float4 *d4 = (const float4 *)(part_of(b) + 2 * ROWS) + d / 4 * ROWS + pr;
+                            float4 y[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = __ldcg(d4 + i * ROWS);
                             const float mb = __ldcg(part_of(b) + pr), f = mb == -INFINITY ? 0.f : ex2(mb - mm);
                             if (f == 0.f) continue;
-                            const float4 *d4 = (const float4 *)(part_of(b) + 2 * ROWS) + d / 4 * ROWS + pr;
-                            float4 y[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) y[i] = __ldcg(d4 + i * ROWS);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
+                            for (int i = 0; i < 16; ++i) {
                                 float *z = x[i / 2] + (i & 1) * 4;
                                 z[0] = fmaf(y[i].x, f, z[0]), z[1] = fmaf(y[i].y, f, z[1]), z[2] = fmaf(y[i].z, f, z[2]), z[3] = fmaf(y[i].w, f, z[3]);
                             }
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) put(d + i * 8, x[i], inv);
+                        for (int i = 0; i < 8; ++i) put(d + i * 8, x[i], inv);
                     }
                 }
             }
-            at = at_next;
-            q = q_next;
-            s = s_next;
+            give_back(seg_i++);
+            seg = next;
+            factor = factor_next;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else if (warp < MMA_WARP) {
@@ -593,17 +630,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         const int sub_row = DP == 64 ? lane >> 2 : (lane >> 4) * 2 + (lane >> 2 & 1);
         const bool takes = cc * 16 < c.dim;
         const int64_t lane_at = sub_row * c.s_slot, per_step = PER * c.s_slot;
-        uint32_t tile_i = 0;
-        int64_t at = line.begin;
+        uint32_t tile_i = 0, seg_i = 0;
         bool ok = true;
-        while (at < line.stop && ok) {
-            const place_t q = find_item<ROWS>(p, line, at);
-            const seq_t s = line.s;
-            const int u0 = (int)(at - q.item_begin), u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
-            const int end = q.item.tokens;
-            if (w == 0 && lane == 0 && u0 == 0 && (int64_t)s.first + (s.end - s.begin) > line.capacity) flag_bad_page(c);
-            const int32_t *table = c.table + (int64_t)line.seq * c.table_s0;
-            const uint8_t *keys = (const uint8_t *)c.key + q.head * c.s_head + cc * 16, *values = (const uint8_t *)c.value + q.head * c.s_head + cc * 16;
+        while (ok) {
+            const segment_t *seg = take(seg_i);
+            if (!seg || seg->rows == 0) break;
+            const int u0 = seg->u0, u1 = seg->u1, end = seg->tokens, head = seg->head;
+            if (w == 0 && lane == 0 && u0 == 0 && seg->over) flag_bad_page(c);
+            const int32_t *table = c.table + (int64_t)seg->seq * c.table_s0;
+            give_back(seg_i++);
+            const uint8_t *keys = (const uint8_t *)c.key + head * c.s_head + cc * 16, *values = (const uint8_t *)c.value + head * c.s_head + cc * 16;
             uint4 kr[LOADS], vr[LOADS];
             // every warp looks up all eight runs of a tile, one per lane, because `ref` needs all their scales
             int64_t place = -1;
@@ -616,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     const int phys = table[n];
                     if (phys >= 0 && phys < c.pages) {
                         place = (int64_t)phys * c.s_page + (int64_t)slot * c.s_slot;
-                        const int64_t i = (int64_t)phys * c.heads + q.head;
+                        const int64_t i = (int64_t)phys * c.heads + head;
                         ks = c.key_scale[i], vs = c.value_scale[i];
                     } else {
                         flag_bad_page(c);
@@ -692,7 +728,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 if (lane == 0) mbar_arrive(&ctrl->v_full[st]);
                 load(j + 1, values, vr);
             }
-            at = q.item_begin + u1;
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MMA_REGS));
@@ -704,8 +739,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         constexpr uint32_t IDESC_O = IDESC | (1u << 16) | ((uint32_t)(DP >> 3) << 17); // values are N-major
         const uint64_t q_desc = make_desc(smem_u32(smem_q), 16, 1024), k_desc = make_desc(smem_u32(smem_k), 16, 1024);
         const uint64_t v_desc = make_desc(smem_u32(smem_v), UNIT * 128, 1024);
-        uint32_t q_phase = 0, p_phase = 0, tile_i = 0; // a bit per tile
-        int64_t at = line.begin;
+        uint32_t q_phase = 0, p_phase = 0; // a bit per tile
+        uint32_t tile_i = 0, seg_i = 0;
         bool ok = true;
         auto scores = [&](int t, int st) { // S_t = Q_t K^T
             const uint64_t a = q_desc + (uint64_t)(t * (S::MAT >> 4)), b = k_desc + (uint64_t)(st * (S::MAT >> 4));
@@ -733,12 +768,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         auto commit = [&](uint64_t *bar) {
             if (elect_one()) tc_commit(bar);
         };
-        while (warp == MMA_WARP && at < line.stop && ok) {
-            const place_t q = find_item<ROWS>(p, line, at);
-            const seq_t s = line.s;
-            const int u0 = (int)(at - q.item_begin), u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
-            const int rows = (s.end - s.begin) * group - q.tile * ROWS, n = u1 - u0;
-            const bool two = rows > TILE;
+        while (warp == MMA_WARP && ok) {
+            const segment_t *seg = take(seg_i);
+            if (!seg || seg->rows == 0) break;
+            const int n = seg->u1 - seg->u0;
+            const bool two = seg->rows > TILE;
+            give_back(seg_i++);
             if (!(ok = warp_wait(&ctrl->k_full[tile_i % STAGES], (tile_i / STAGES) & 1, ctrl, status))) break;
             if (!(ok = warp_wait(&ctrl->q_full[0], q_phase & 1, ctrl, status))) break;
             q_phase ^= 1;
@@ -771,7 +806,41 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 commit(&ctrl->v_empty[st]);
                 if (!last) commit(&ctrl->k_empty[next]);
             }
-            at = q.item_begin + u1;
+        }
+        if (warp == MMA_WARP + 1) {
+            // ---------------- the segments ----------------
+            int64_t at = line.begin;
+            for (uint32_t i = 0;; ++i) {
+                segment_t g;
+                g.rows = 0;
+                const bool more = at < line.stop;
+                if (more) {
+                    const place_t q = find_item<ROWS>(p, line, at);
+                    g.begin = line.s.begin;
+                    g.row0 = q.tile * ROWS;
+                    g.rows = (line.s.end - line.s.begin) * group - g.row0;
+                    g.first = line.s.first;
+                    g.head = q.head;
+                    g.seq = line.seq;
+                    g.tokens = q.item.tokens;
+                    g.u0 = (int)(at - q.item_begin);
+                    g.u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
+                    g.units = q.item.units;
+                    g.c0 = owner(line, q.item_begin);
+                    g.c1 = owner(line, q.item_begin + q.item.units - 1);
+                    g.slot = at == line.begin ? 0 : 1;
+                    g.parity = (int)(part_index(line, q.item_begin, g.c0, g.c0) & 1);
+                    g.over = (int64_t)line.s.first + (line.s.end - line.s.begin) > line.capacity;
+                    at = q.item_begin + g.u1;
+                }
+                if (i >= SEGMENTS && !warp_wait(&ctrl->seg_empty[i % SEGMENTS], (i / SEGMENTS - 1) & 1, ctrl, status)) break;
+                if (lane == 0) {
+                    ctrl->segments[i % SEGMENTS] = g;
+                    mbar_arrive(&ctrl->seg_full[i % SEGMENTS]);
+                }
+                __syncwarp();
+                if (!more) break;
+            }
         }
     }
     // all roles are through (the MMAs too: every one was waited for by way of o_full, unless a wait ran out)

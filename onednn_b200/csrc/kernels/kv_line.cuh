@@ -18,46 +18,46 @@ struct item_t {
     int units;  // one at least: rows that see nothing are still written
 };
 
-// The items of one key head of a sequence, in order; without a division per item.
+// item `tile` of a key head; ones behind the last cost nothing
 template <int ROWS>
-struct items_t {
-    int rows, tokens, group, first, tile = 0;
-    int last, rest;       // ((tile + 1) * ROWS - 1) / group and what is left
-    int step, step_rest;  // ROWS / group and what is left
-    int64_t capacity;
+__device__ __forceinline__ item_t item_of(const seq_t &s, int group, int tile, int64_t capacity) {
+    const int rows = (s.end - s.begin) * group;
+    item_t i = {0, 0};
+    if ((int64_t)tile * ROWS >= rows) return i;
+    const int newest = (min((tile + 1) * ROWS, rows) - 1) / group; // the token of its last row
+    i.tokens = (int)min((int64_t)max(0, s.first + newest + 1), capacity);
+    i.units = max(1, (i.tokens + UNIT - 1) / UNIT);
+    return i;
+}
 
-    __device__ __forceinline__ items_t(const seq_t &s, int group_, int64_t capacity_) {
-        group = group_;
-        capacity = capacity_;
-        first = s.first;
-        tokens = s.end - s.begin;
-        rows = tokens * group;
-        step = ROWS / group;
-        step_rest = ROWS - step * group;
-        last = (ROWS - 1) / group;
-        rest = ROWS - 1 - last * group;
-    }
-    __device__ __forceinline__ bool there() const { return tile * ROWS < rows; }
-    __device__ __forceinline__ item_t get() const {
-        const int newest = min(last, tokens - 1); // token of its last row
-        item_t i;
-        i.tokens = (int)min((int64_t)max(0, first + newest + 1), capacity);
-        i.units = max(1, (i.tokens + UNIT - 1) / UNIT);
-        return i;
-    }
-    __device__ __forceinline__ void next() {
-        ++tile;
-        last += step;
-        rest += step_rest;
-        if (rest >= group) rest -= group, ++last;
-    }
-};
-
-// units of one key head of a sequence
+// units of one key head of a sequence, the lanes of a warp side by side
 template <int ROWS>
-__device__ __forceinline__ int64_t head_units(const seq_t &s, int group, int64_t capacity) {
+__device__ __forceinline__ int64_t head_units_warp(const seq_t &s, int group, int64_t capacity) {
+    const int tiles = ((s.end - s.begin) * group + ROWS - 1) / ROWS;
     int64_t n = 0;
-    for (items_t<ROWS> i(s, group, capacity); i.there(); i.next()) n += i.get().units;
+    for (int tile = threadIdx.x & 31; tile < tiles; tile += 32) n += item_of<ROWS>(s, group, tile, capacity).units;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
+    return n;
+}
+
+// the same for a sequence of its own per lane (`there`: the lane has one): short ones by their lanes, the others by the
+// whole warp, one after the other
+template <int ROWS>
+__device__ __forceinline__ int64_t head_units_lanes(const seq_t &s, bool there, int group, int64_t capacity) {
+    const int tiles = there ? ((s.end - s.begin) * group + ROWS - 1) / ROWS : 0;
+    int64_t n = 0;
+    if (tiles <= 4)
+        for (int tile = 0; tile < tiles; ++tile) n += item_of<ROWS>(s, group, tile, capacity).units;
+    for (uint32_t todo = __ballot_sync(~0u, tiles > 4); todo; todo &= todo - 1) {
+        const int k = __ffs(todo) - 1;
+        seq_t one;
+        one.begin = __shfl_sync(~0u, s.begin, k);
+        one.end = __shfl_sync(~0u, s.end, k);
+        one.first = __shfl_sync(~0u, s.first, k);
+        const int64_t m = head_units_warp<ROWS>(one, group, capacity);
+        if ((int)(threadIdx.x & 31) == k) n = m;
+    }
     return n;
 }
 
@@ -106,8 +106,9 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
     l.total = 0;
     for (int base = 0; base < c.seqs; base += threads) {
         const int b = base + tid;
-        int64_t n = 0;
-        if (b < c.seqs) n = head_units<ROWS>(load_seq(c, b, p.rows), l.group, l.capacity) * l.heads;
+        seq_t s = {0, 0, 0};
+        if (b < c.seqs) s = load_seq(c, b, p.rows);
+        int64_t n = head_units_lanes<ROWS>(s, b < c.seqs, l.group, l.capacity) * l.heads;
         n = block_scan(n, warp_sum);
         if (tid == threads - 1) words[0] = n;
         __syncthreads();
@@ -122,8 +123,9 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
     l.seq_begin = 0;
     for (int base = 0; base < c.seqs; base += threads) {
         const int b = base + tid;
-        int64_t n = 0;
-        if (b < c.seqs) n = head_units<ROWS>(load_seq(c, b, p.rows), l.group, l.capacity) * l.heads;
+        seq_t s = {0, 0, 0};
+        if (b < c.seqs) s = load_seq(c, b, p.rows);
+        const int64_t n = head_units_lanes<ROWS>(s, b < c.seqs, l.group, l.capacity) * l.heads;
         const int64_t upto = l.seq_begin + block_scan(n, warp_sum);
         __syncthreads();
         if (tid == 0) words[0] = -1;
@@ -140,30 +142,50 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
         __syncthreads();
     }
     l.s = load_seq(c, l.seq, p.rows);
-    l.per_head = head_units<ROWS>(l.s, l.group, l.capacity);
+    l.per_head = head_units_warp<ROWS>(l.s, l.group, l.capacity);
     return true;
 }
 
-// the item at unit `at`, which never goes back
+// the item at unit `at`, which never goes back; whole warps
 template <int ROWS>
 __device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p, part_t &l, int64_t at) {
     while (at - l.seq_begin >= l.per_head * l.heads) {
         l.seq_begin += l.per_head * l.heads;
         l.s = load_seq(p.cache, ++l.seq, p.rows);
-        l.per_head = head_units<ROWS>(l.s, l.group, l.capacity);
+        l.per_head = head_units_warp<ROWS>(l.s, l.group, l.capacity);
     }
     place_t q;
     q.head = (int)((at - l.seq_begin) / l.per_head);
     q.item_begin = l.seq_begin + q.head * l.per_head;
-    items_t<ROWS> i(l.s, l.group, l.capacity);
-    q.item = i.get();
-    while (at - q.item_begin >= q.item.units) {
-        q.item_begin += q.item.units;
-        i.next();
-        q.item = i.get();
+    const int lane = threadIdx.x & 31;
+    q.tile = 0;
+    if ((l.s.end - l.s.begin) * l.group <= 4 * ROWS) { // few items: one after the other
+        q.item = item_of<ROWS>(l.s, l.group, 0, l.capacity);
+        while (at - q.item_begin >= q.item.units) {
+            q.item_begin += q.item.units;
+            q.item = item_of<ROWS>(l.s, l.group, ++q.tile, l.capacity);
+        }
+        return q;
     }
-    q.tile = i.tile;
-    return q;
+    for (;; q.tile += 32) { // 32 items at a time
+        const item_t mine = item_of<ROWS>(l.s, l.group, q.tile + lane, l.capacity);
+        int64_t upto = mine.units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(~0u, upto, o);
+            if (lane >= o) upto += u;
+        }
+        const uint32_t here = __ballot_sync(~0u, at - q.item_begin < upto);
+        if (here) {
+            const int k = __ffs(here) - 1;
+            q.tile += k;
+            q.item.tokens = __shfl_sync(~0u, mine.tokens, k);
+            q.item.units = __shfl_sync(~0u, mine.units, k);
+            q.item_begin += __shfl_sync(~0u, upto, k) - q.item.units;
+            return q;
+        }
+        q.item_begin += __shfl_sync(~0u, upto, 31);
+    }
 }
 
 // the block whose part holds unit u
