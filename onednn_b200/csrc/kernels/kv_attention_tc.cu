@@ -2,17 +2,18 @@
 // Bound by the tensor cores and, next to them, by the exponentials.
 //
 // A work item (kv_line.cuh) has 256 query rows, tokens x the query heads of a key head, in two tiles of 128, so that a
-// tile of keys and values is converted once for 256 rows.  Per 128 tokens and tile t, on tcgen05.mma (f16 in,
+// tile of keys and values is converted once for 256 rows.  Per step of 64 tokens and tile t, on tcgen05.mma (f16 in,
 // f32 accumulators in tensor memory):
-//   S_t = Q_t K^T        128 x 128 x dim, both operands in shared memory, K-major
-//   O_t += P_t V         128 x dim x 128, P from tensor memory (over S, where it was computed), V as it lies, N-major
+//   S_t = Q_t K^T        128 x 64 x dim, both operands in shared memory, K-major
+//   O_t += P_t V         128 x dim x 64, P from tensor memory (over S, where it was computed), V as it lies, N-major
+// S_t has two places, so that a step's scores are there before the softmax is through with the step before; with one
+// place of 128 tokens the softmax waited a third of the time for the products between.
 //
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row, so maximum and sum need no exchange; queries
 //                    on the way in, results on the way out
 //   warps 8-11       codes from the pages to f16 tiles in shared memory (exact), a tile ahead in registers
 //   warp 13          finds the block's items ahead of all others and lays them out in shared memory
-//   warp 12          one thread issues all MMAs: QK_0(j+1) behind PV_0(j), QK_1(j+1) behind PV_1(j), so that one
-//                    tile's softmax runs beside the other's products
+//   warp 12          one thread issues all MMAs: for each tile PV(s), then the scores of step s + 2 into the same place
 //
 // The two scales stay out of the products.  A page holds a multiple of 16 tokens here, so 16 neighbouring tokens share
 // theirs: x = s * (key scale * softmax scale), and the value scale enters the exponent,
@@ -37,6 +38,7 @@ constexpr int REGS = 128, SOFTMAX_REGS = 176, CONVERT_REGS = 104, MMA_REGS = 56;
 static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * REGS && THREADS * REGS <= 65536, "");
 constexpr int STAGES = 2;  // of keys and of values
 constexpr int CHUNKS = UNIT / 16;
+constexpr int STEP = 64, STEPS = UNIT / STEP; // tokens of a step; steps of a unit, which the converters work on
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t WAIT_TRIES = 1u << 19; // of up to 2 us each, suspended in hardware
 enum : uint32_t { ST_WAIT = 0x00100000 };
@@ -76,7 +78,7 @@ constexpr int SEGMENTS = 4;
 struct ctrl_t {
     uint64_t seg_full[SEGMENTS], seg_empty[SEGMENTS];
     segment_t segments[SEGMENTS];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], join;
+    uint64_t q_full[2], s_full[2][STEPS], p_full[2][STEPS], o_done[2][STEPS], join;
     uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
     uint32_t tmem_base;
     volatile uint32_t abort;
@@ -159,16 +161,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
     tmem_ld32_issue(addr, v);
     tmem_ld32_wait(v);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
-    asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-            "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-            "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
-            "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
-            "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
-            "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
-            : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
     asm volatile(
             "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
@@ -189,6 +181,11 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&v)[16]) {
                  : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
                  "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
                  :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -277,9 +274,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctrl->q_full[i], SOFTMAX_WARPS / 2);
-            mbar_init(&ctrl->p_full[i], SOFTMAX_WARPS / 2);
-            mbar_init(&ctrl->s_full[i], 1);
-            mbar_init(&ctrl->o_full[i], 1);
+            for (int b = 0; b < STEPS; ++b) {
+                mbar_init(&ctrl->p_full[i][b], SOFTMAX_WARPS / 2);
+                mbar_init(&ctrl->s_full[i][b], 1);
+                mbar_init(&ctrl->o_done[i][b], 1);
+            }
         }
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&ctrl->k_full[i], CONVERT_WARPS);
@@ -311,6 +310,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     auto take = [&](uint32_t i) -> const segment_t * {
         return warp_wait(&ctrl->seg_full[i % SEGMENTS], (i / SEGMENTS) & 1, ctrl, status) ? &ctrl->segments[i % SEGMENTS] : nullptr;
     };
+    // steps of a segment: up to its last token, one at least
+    auto steps_of = [&](const segment_t &g) { return max(1, min(g.u1 * STEPS, (g.tokens + STEP - 1) / STEP) - g.u0 * STEPS); };
     auto give_back = [&](uint32_t i) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctrl->seg_empty[i % SEGMENTS]);
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         const bool bf16 = p.query_dt == B200_DT_BF16;
         float *parts = (float *)((char *)p.scratch + counter_bytes(gridDim.x));
         constexpr size_t part_size = (size_t)ROWS * (DP + 2);
-        uint32_t s_phase = 0, o_phase = 0, tile_i = 0; // tile_i: tiles of tokens since the launch
+        uint32_t s_phase = 0, o_phase = 0, tile_i = 0; // phases: a bit per place; units since the launch
         bool ok = true;
         uint32_t join_phase = 0;
         auto join = [&]() { // all softmax warps
@@ -409,123 +410,111 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             if (active) {
                 const int limit = mine ? seg->first + (seg->row0 + t * TILE + r) / group : -1;
                 const int first_limit = __shfl_sync(~0u, limit, 0); // the smallest of the warp's rows that exist
-                for (int j = u0; j < u1; ++j, ++tile_i) {
-                    if (!(ok = warp_wait(&ctrl->s_full[t], s_phase, ctrl, status))) break;
-                    s_phase ^= 1;
+                const int steps = steps_of(*seg);
+                // the latest products with the weights in `place` (two may be under way, one per place)
+                auto products_done = [&](int place) { return warp_wait(&ctrl->o_done[t][place], (o_phase >> place & 1) ^ 1, ctrl, status); };
+                for (int j = 0; j < steps; ++j) {
+                    const int place = j % STEPS;
+                    if (!(ok = warp_wait(&ctrl->s_full[t][place], s_phase >> place & 1, ctrl, status))) break;
+                    s_phase ^= 1u << place;
                     tc_fence_after();
-                    if (j + 1 == u1) fetch_next();
-                    const scales_t &sc = ctrl->scales[tile_i & 3];
-                    uint32_t va[32], vb[32];
-                    if (j * UNIT + UNIT - 1 > first_limit) { // the last tiles: what a row does not see goes from its scores
-                        const int seen = limit - j * UNIT;   // columns 0 .. seen are seen
-#pragma unroll 1
-                        for (int h = 0; h < UNIT / 32; ++h) {
-                            tmem_ld32(tmem_s + h * 32, va);
+                    if (j + 1 == steps) fetch_next();
+                    const scales_t &sc = ctrl->scales[(tile_i + j / STEPS) & 3];
+                    const float4 *chunk = sc.chunk + place * (STEP / 16);
+                    const uint32_t tmem_p = tmem_s + place * STEP;
+                    // ---- the scores, and the largest
+                    uint32_t v[2][32];
+                    float4 ck[4];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (h * 32 + i > seen) va[i] = 0xff800000u;
-                            tmem_st32(tmem_s + h * 32, va);
-                        }
-                        tmem_wait_st();
+                    for (int k = 0; k < 4; ++k) ck[k] = chunk[k];
+                    const float step = place == 0 ? sc.step : 1.f;
+                    up = sc.up;
+                    tmem_ld32_issue(tmem_p, v[0]);
+                    tmem_ld32_issue(tmem_p + 32, v[1]);
+                    tmem_ld32_wait(v[0]);
+                    tmem_ld32_wait(v[1]);
+                    if (u0 * UNIT + j * STEP + STEP - 1 > first_limit) { // the last steps: what a row does not see goes from its scores
+                        const int seen = limit - u0 * UNIT - j * STEP;   // columns 0 .. seen are seen
+#pragma unroll
+                        for (int i = 0; i < STEP; ++i)
+                            if (i > seen) v[i >> 5][i & 31] = 0xff800000u;
                     }
-                    tmem_ld32_issue(tmem_s, va);
-                    // O, the sum and the weights of this tile that are stored already (`done` columns) follow m and ref
-                    auto rescale = [&](float d, float fo, int done) {
-                        tmem_wait_st(); // what was stored is read here
+                    float f[4], top = m;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t *y = v[k >> 1] + (k & 1) * 16;
+                        float x0 = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
+                        float x1 = max3(__uint_as_float(y[8]), __uint_as_float(y[9]), __uint_as_float(y[10]));
+#pragma unroll
+                        for (int i = 3; i < 7; i += 2) {
+                            x0 = max3(x0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+                            x1 = max3(x1, __uint_as_float(y[8 + i]), __uint_as_float(y[9 + i]));
+                        }
+                        x0 = max3(x0, x1, __uint_as_float(y[7]));
+                        f[k] = ck[k].x * factor;
+                        top = fmaxf(top, fmaf(fmaxf(x0, __uint_as_float(y[15])), f[k], ck[k].y));
+                    }
+                    // ---- m and ref follow, seldom; O and the sum with them
+                    const bool follow = top > m + 8.f; // also from -inf
+                    if (__any_sync(~0u, follow || step != 1.f)) {
+                        const float d = follow ? ex2(m - top) : 1.f, fo = d * step;
+                        if (follow) m = top;
                         l *= d;
-                        if (j > u0) {
+                        if (j > 0) { // the products of the step before are added up first
+                            if (!(ok = products_done(place ^ 1))) break;
+                            tc_fence_after();
 #pragma unroll 1
                             for (int h = 0; h < DP / 16; ++h) {
-                                uint32_t v[16];
-                                tmem_ld16(tmem_o + h * 16, v);
+                                uint32_t w[16];
+                                tmem_ld16(tmem_o + h * 16, w);
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * fo);
-                                tmem_st16(tmem_o + h * 16, v);
+                                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * fo);
+                                tmem_st16(tmem_o + h * 16, w);
                             }
                         }
-#pragma unroll 1
-                        for (int h = 0; h < done; h += FINE ? 16 : 32) {
-                            uint32_t v[16];
-                            tmem_ld16(tmem_s + h, v);
-                            const uint32_t dd = pack_f16x2(d, d);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(v[i]) : "r"(dd));
-                            tmem_st16(tmem_s + h, v);
-                        }
-                    };
-                    up = sc.up;
-                    if (sc.step != 1.f && j > u0) { // the same for all rows
-                        tmem_ld32_wait(va);
-                        rescale(1.f, sc.step, 0);
                     }
-                    // 32 columns: the largest score, m where that has outgrown it, the weights over the scores
-                    auto columns = [&](int h, uint32_t (&v)[32], uint32_t (&next)[32]) {
-                        tmem_ld32_wait(v);
-                        if (h + 1 < UNIT / 32) tmem_ld32_issue(tmem_s + (h + 1) * 32, next);
-                        const float4 c0 = sc.chunk[2 * h], c1 = sc.chunk[2 * h + 1];
-                        const float f0 = c0.x * factor, f1 = c1.x * factor;
-                        float x0 = max3(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]));
-                        float x1 = max3(__uint_as_float(v[16]), __uint_as_float(v[17]), __uint_as_float(v[18]));
+                    // ---- weights, over the scores: of each 16 columns the first eight, FINE: the other eight too
+                    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                        for (int i = 3; i < 15; i += 2) {
-                            x0 = max3(x0, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                            x1 = max3(x1, __uint_as_float(v[16 + i]), __uint_as_float(v[17 + i]));
-                        }
-                        const float top = fmaxf(fmaf(fmaxf(x0, __uint_as_float(v[15])), f0, c0.y), fmaf(fmaxf(x1, __uint_as_float(v[31])), f1, c1.y));
-                        if (__any_sync(~0u, top > m + 8.f)) { // also from -inf
-                            const float m_now = top > m + 8.f ? top : m;
-                            const float d = m_now == m ? 1.f : ex2(m - m_now);
-                            if (h + 1 < UNIT / 32) tmem_ld32_wait(next);
-                            rescale(d, d, h * 32);
-                            m = m_now;
-                        }
-                        const float base = m == -INFINITY ? 0.f : m;
-                        uint32_t pw[16], rest[FINE ? 16 : 1];
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t *y = v[k >> 1] + (k & 1) * 16;
+                        const float off = ck[k].z - base;
+                        const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(off, off);
+                        uint64_t sum = 0;
+                        uint32_t pw[FINE ? 16 : 8];
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float off = (k ? c1.z : c0.z) - base;
-                            const uint64_t ff = f32x2(k ? f1 : f0, k ? f1 : f0), oo = f32x2(off, off);
-                            uint64_t sum = 0;
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const float2 x = unpack2(fma2(f32x2(__uint_as_float(v[k * 16 + i]), __uint_as_float(v[k * 16 + i + 1])), ff, oo));
-                                const float e0 = ex2(x.x), e1 = ex2(x.y);
-                                sum = add2(sum, f32x2(e0, e1));
-                                const uint32_t hi = pack_f16x2(e0, e1);
-                                pw[k * 8 + i / 2] = hi;
-                                if (FINE) {
-                                    const float2 had = f16x2_to_f32(hi);
-                                    rest[FINE ? k * 8 + i / 2 : 0] = pack_f16x2(e0 - had.x, e1 - had.y);
-                                }
+                        for (int i = 0; i < 16; i += 2) {
+                            const float2 x = unpack2(fma2(f32x2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), ff, oo));
+                            const float e0 = ex2(x.x), e1 = ex2(x.y);
+                            sum = add2(sum, f32x2(e0, e1));
+                            const uint32_t hi = pack_f16x2(e0, e1);
+                            pw[i / 2] = hi;
+                            if (FINE) {
+                                const float2 had = f16x2_to_f32(hi);
+                                pw[FINE ? 8 + i / 2 : 0] = pack_f16x2(e0 - had.x, e1 - had.y);
                             }
-                            const float2 both = unpack2(sum);
-                            l = fmaf(both.x + both.y, k ? c1.w : c0.w, l);
                         }
-                        // over the columns just read; the first half, or both
-                        tmem_st16(tmem_s + h * 32, pw);
-                        if (FINE) tmem_st16(tmem_s + h * 32 + 16, rest);
-                    };
-#pragma unroll 1
-                    for (int h = 0; h < UNIT / 32; h += 2) {
-                        columns(h, va, vb);
-                        columns(h + 1, vb, va);
+                        const float2 both = unpack2(sum);
+                        l = fmaf(both.x + both.y, ck[k].w, l);
+                        if (FINE) tmem_st16(tmem_p + k * 16, pw);
+                        else tmem_st8(tmem_p + k * 16, pw);
                     }
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctrl->p_full[t]);
+                    if (lane == 0) mbar_arrive(&ctrl->p_full[t][place]);
+                    o_phase ^= 1u << place;
                 }
                 if (ok) {
                     prepare_next(); // beside the last products
-                    ok = warp_wait(&ctrl->o_full[t], o_phase, ctrl, status);
+                    ok = products_done((steps - 1) % STEPS);
+                    tc_fence_after();
                 }
-                o_phase ^= 1;
-                tc_fence_after();
             } else {
-                tile_i += (uint32_t)(u1 - u0);
                 fetch_next();
                 prepare_next();
             }
+            tile_i += (uint32_t)(u1 - u0);
 
             // ---- the row's result, or its part of it
             const bool whole = u0 == 0 && u1 == seg->units;
@@ -689,44 +678,52 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 }
             };
             float ref = -200.f;
-            find(u0);
-            load(u0, keys, kr);
-            load(u0, values, vr);
-            for (int j = u0; j < u1; ++j, ++tile_i) {
-                const int st = tile_i % STAGES;
-                const uint32_t use = tile_i / STAGES;
-                // keys, and both scales: a softmax that sees the scores sees them
-                if (use > 0 && !(ok = warp_wait(&ctrl->k_empty[st], (use - 1) & 1, ctrl, status))) break;
-                {
-                    const float log = lg2(fmaxf(vs, 7.5231638e-37f)); // 2^-120 at least
-                    float top = lane < CHUNKS ? log : -200.f;
+            // keys of unit j (the i-th since the launch), and both scales: a softmax that sees the scores sees them
+            auto put_keys = [&](uint32_t i) {
+                const int st = i % STAGES;
+                const uint32_t use = i / STAGES;
+                if (use > 0 && !(ok = warp_wait(&ctrl->k_empty[st], (use - 1) & 1, ctrl, status))) return;
+                const float log = lg2(fmaxf(vs, 7.5231638e-37f)); // 2^-120 at least
+                float top = lane < CHUNKS ? log : -200.f;
 #pragma unroll
-                    for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-                    top = __shfl_sync(~0u, top, 0);
-                    // with room, so that it seldom moves
-                    const float now = top > ref ? ceilf(top) + 1.f : ref;
-                    if (w == 0 && lane < CHUNKS) {
-                        scales_t &sc = ctrl->scales[tile_i & 3];
-                        const bool there = ks >= 0.f;
-                        // scales below 2^-60 of the largest count as that: their values round to nothing, their weights stay in the sum
-                        const float z = fmaxf(log - now, -60.f);
-                        sc.chunk[lane] = make_float4(fmaxf(ks, SMALL), there ? 0.f : -INFINITY, there ? z : -INFINITY, ex2(-z));
-                        if (lane == 0) sc.step = now == ref ? 1.f : ex2(ref - now), sc.up = ex2(now);
-                    }
-                    ref = now;
+                for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+                top = __shfl_sync(~0u, top, 0);
+                // with room, so that it seldom moves
+                const float now = top > ref ? ceilf(top) + 1.f : ref;
+                if (w == 0 && lane < CHUNKS) {
+                    scales_t &sc = ctrl->scales[i & 3];
+                    const bool there = ks >= 0.f;
+                    // scales below 2^-60 of the largest count as that: their values round to nothing, their weights stay in the sum
+                    const float z = fmaxf(log - now, -60.f);
+                    sc.chunk[lane] = make_float4(fmaxf(ks, SMALL), there ? 0.f : -INFINITY, there ? z : -INFINITY, ex2(-z));
+                    if (lane == 0) sc.step = now == ref ? 1.f : ex2(ref - now), sc.up = ex2(now);
                 }
+                ref = now;
                 convert(kr, smem_k + st * S::MAT);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->k_full[st]);
-                find(j + 1);
-                load(j + 1, keys, kr);
+            };
+            // the keys go a unit ahead of the values: the scores are computed that much ahead of the products
+            find(u0);
+            load(u0, keys, kr);
+            load(u0, values, vr);
+            put_keys(tile_i);
+            find(u0 + 1);
+            load(u0 + 1, keys, kr);
+            for (int j = u0; j < u1 && ok; ++j, ++tile_i) {
+                if (j + 1 < u1) put_keys(tile_i + 1);
+                if (!ok) break;
+                const int st = tile_i % STAGES;
+                const uint32_t use = tile_i / STAGES;
                 if (use > 0 && !(ok = warp_wait(&ctrl->v_empty[st], (use - 1) & 1, ctrl, status))) break;
                 convert(vr, smem_v + st * S::MAT);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->v_full[st]);
                 load(j + 1, values, vr);
+                find(j + 2);
+                load(j + 2, keys, kr);
             }
         }
     } else {
@@ -735,34 +732,34 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         // The whole warp walks through the loops, so that descriptors and addresses are uniform values; one lane
         // issues.  Tensor memory addresses are constants: the kernel allocates all columns.
         constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(TILE >> 4) << 24);
-        constexpr uint32_t IDESC_S = IDESC | ((uint32_t)(UNIT >> 3) << 17);
+        constexpr uint32_t IDESC_S = IDESC | ((uint32_t)(STEP >> 3) << 17);
         constexpr uint32_t IDESC_O = IDESC | (1u << 16) | ((uint32_t)(DP >> 3) << 17); // values are N-major
         const uint64_t q_desc = make_desc(smem_u32(smem_q), 16, 1024), k_desc = make_desc(smem_u32(smem_k), 16, 1024);
         const uint64_t v_desc = make_desc(smem_u32(smem_v), UNIT * 128, 1024);
-        uint32_t q_phase = 0, p_phase = 0; // a bit per tile
+        uint32_t q_phase = 0, p_phase = 0; // a bit per tile; per tile and place
         uint32_t tile_i = 0, seg_i = 0;
         bool ok = true;
-        auto scores = [&](int t, int st) { // S_t = Q_t K^T
-            const uint64_t a = q_desc + (uint64_t)(t * (S::MAT >> 4)), b = k_desc + (uint64_t)(st * (S::MAT >> 4));
+        auto scores = [&](int t, int st, int place) { // S_t = Q_t K^T, the place's half of a unit
+            const uint64_t a = q_desc + (uint64_t)(t * (S::MAT >> 4)), b = k_desc + (uint64_t)((st * S::MAT + place * STEP * 128) >> 4);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
                     const uint32_t o = (uint32_t)((k >> 2) * (UNIT * 128) + (k & 3) * 32) >> 4;
-                    mma_ss(t * UNIT, a + o, b + o, IDESC_S, k != 0);
+                    mma_ss(t * UNIT + place * STEP, a + o, b + o, IDESC_S, k != 0);
                 }
-                tc_commit(&ctrl->s_full[t]);
+                tc_commit(&ctrl->s_full[t][place]);
             }
         };
-        auto weigh = [&](int t, int st, bool more, bool last) { // O_t += P_t V
-            const uint64_t b = v_desc + (uint64_t)(st * (S::MAT >> 4));
+        auto weigh = [&](int t, int st, int place, bool more) { // O_t += P_t V
+            const uint64_t b = v_desc + (uint64_t)((st * S::MAT + place * STEP * 128) >> 4);
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < UNIT / 16; ++k) {
-                    const uint32_t a = t * UNIT + (k >> 1) * 32 + (k & 1) * 8;
+                for (int k = 0; k < STEP / 16; ++k) {
+                    const uint32_t a = t * UNIT + place * STEP + k * 16;
                     mma_ts(2 * UNIT + t * DP, a, b + k * (2048 >> 4), IDESC_O, more || k != 0);
-                    if (FINE) mma_ts(2 * UNIT + t * DP, a + 16, b + k * (2048 >> 4), IDESC_O, 1);
+                    if (FINE) mma_ts(2 * UNIT + t * DP, a + 8, b + k * (2048 >> 4), IDESC_O, 1);
                 }
-                if (last) tc_commit(&ctrl->o_full[t]);
+                tc_commit(&ctrl->o_done[t][place]);
             }
         };
         auto commit = [&](uint64_t *bar) {
@@ -771,41 +768,40 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         while (warp == MMA_WARP && ok) {
             const segment_t *seg = take(seg_i);
             if (!seg || seg->rows == 0) break;
-            const int n = seg->u1 - seg->u0;
+            const int n = steps_of(*seg), units = seg->u1 - seg->u0;
             const bool two = seg->rows > TILE;
             give_back(seg_i++);
-            if (!(ok = warp_wait(&ctrl->k_full[tile_i % STAGES], (tile_i / STAGES) & 1, ctrl, status))) break;
-            if (!(ok = warp_wait(&ctrl->q_full[0], q_phase & 1, ctrl, status))) break;
-            q_phase ^= 1;
-            tc_fence_after();
-            scores(0, tile_i % STAGES);
-            if (two) {
-                if (!(ok = warp_wait(&ctrl->q_full[1], q_phase >> 1, ctrl, status))) break;
-                q_phase ^= 2;
+            auto stage = [&](int s) { return (int)((tile_i + s / STEPS) % STAGES); };
+            auto use = [&](int s) { return (tile_i + s / STEPS) / STAGES & 1; };
+            if (!(ok = warp_wait(&ctrl->k_full[stage(0)], use(0), ctrl, status))) break;
+            for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
+                if (!(ok = warp_wait(&ctrl->q_full[t], q_phase >> t & 1, ctrl, status))) break;
+                q_phase ^= 1u << t;
                 tc_fence_after();
-                scores(1, tile_i % STAGES);
+                scores(t, stage(0), 0);
+                if (n > 1) scores(t, stage(0), 1);
             }
-            commit(&ctrl->k_empty[tile_i % STAGES]);
-            for (int j = 0; j < n; ++j, ++tile_i) {
-                const int st = tile_i % STAGES, next = (tile_i + 1) % STAGES;
-                const bool last = j + 1 == n;
-                if (!(ok = warp_wait(&ctrl->v_full[st], (tile_i / STAGES) & 1, ctrl, status))) break;
-                if (!last && !(ok = warp_wait(&ctrl->k_full[next], ((tile_i + 1) / STAGES) & 1, ctrl, status))) break;
-                if (!(ok = warp_wait(&ctrl->p_full[0], p_phase & 1, ctrl, status))) break;
-                p_phase ^= 1;
-                tc_fence_after();
-                weigh(0, st, j > 0, last);
-                if (!last) scores(0, next);
-                if (two) {
-                    if (!(ok = warp_wait(&ctrl->p_full[1], p_phase >> 1, ctrl, status))) break;
-                    p_phase ^= 2;
-                    tc_fence_after();
-                    weigh(1, st, j > 0, last);
-                    if (!last) scores(1, next);
+            if (!ok) break;
+            commit(&ctrl->k_empty[stage(0)]);
+            for (int s = 0; s < n; ++s) {
+                const int place = s % STEPS;
+                if (place == 0) {
+                    if (!(ok = warp_wait(&ctrl->v_full[stage(s)], use(s), ctrl, status))) break;
+                    if (s + 2 < n && !(ok = warp_wait(&ctrl->k_full[stage(s + 2)], use(s + 2), ctrl, status))) break;
                 }
-                commit(&ctrl->v_empty[st]);
-                if (!last) commit(&ctrl->k_empty[next]);
+                for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
+                    const int bit = t * STEPS + place;
+                    if (!(ok = warp_wait(&ctrl->p_full[t][place], p_phase >> bit & 1, ctrl, status))) break;
+                    p_phase ^= 1u << bit;
+                    tc_fence_after();
+                    weigh(t, stage(s), place, s > 0);
+                    if (s + 2 < n) scores(t, stage(s + 2), place);
+                }
+                if (!ok) break;
+                if (place == 1 || s + 1 == n) commit(&ctrl->v_empty[stage(s)]);
+                if (s + 2 < n && (place == 1 || s + 3 == n)) commit(&ctrl->k_empty[stage(s + 2)]);
             }
+            tile_i += (uint32_t)units;
         }
         if (warp == MMA_WARP + 1) {
             // ---------------- the segments ----------------
@@ -843,7 +839,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             }
         }
     }
-    // all roles are through (the MMAs too: every one was waited for by way of o_full, unless a wait ran out)
+    // all roles are through (the MMAs too: every one was waited for by way of o_done, unless a wait ran out)
     __syncthreads();
     if (warp == MMA_WARP) {
         tc_fence_after();
