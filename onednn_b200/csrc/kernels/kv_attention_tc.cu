@@ -12,8 +12,10 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row, so maximum and sum need no exchange; queries
 //                    on the way in, results on the way out
 //   warps 8-11       codes from the pages to f16 tiles in shared memory (exact), a tile ahead in registers
-//   warp 13          finds the block's items ahead of all others and lays them out in shared memory
-//   warp 12          one thread issues all MMAs: for each tile PV(s), then the scores of step s + 2 into the same place
+//   warps 12, 13     one thread of each issues the MMAs of tile 0, 1: PV(s), then the scores of step s + 2 into the same
+//                    place.  (One thread for both tiles was what everything waited for: an MMA takes it some 70 cycles, a
+//                    look at a barrier some 300.)
+//   warp 14          finds the block's items ahead of all others and lays them out in shared memory
 //
 // The two scales stay out of the products.  A page holds a multiple of 16 tokens here, so 16 neighbouring tokens share
 // theirs: x = s * (key scale * softmax scale), and the value scale enters the exponent,
@@ -283,12 +285,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(&ctrl->k_full[i], CONVERT_WARPS);
             mbar_init(&ctrl->v_full[i], CONVERT_WARPS);
-            mbar_init(&ctrl->k_empty[i], 1);
-            mbar_init(&ctrl->v_empty[i], 1);
+            mbar_init(&ctrl->k_empty[i], 2); // both issuers
+            mbar_init(&ctrl->v_empty[i], 2);
         }
         for (int i = 0; i < SEGMENTS; ++i) {
             mbar_init(&ctrl->seg_full[i], 1);
-            mbar_init(&ctrl->seg_empty[i], SOFTMAX_WARPS + CONVERT_WARPS + 1);
+            mbar_init(&ctrl->seg_empty[i], SOFTMAX_WARPS + CONVERT_WARPS + 2);
         }
         mbar_init(&ctrl->join, SOFTMAX_WARPS);
         ctrl->abort = 0;
@@ -736,10 +738,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         constexpr uint32_t IDESC_O = IDESC | (1u << 16) | ((uint32_t)(DP >> 3) << 17); // values are N-major
         const uint64_t q_desc = make_desc(smem_u32(smem_q), 16, 1024), k_desc = make_desc(smem_u32(smem_k), 16, 1024);
         const uint64_t v_desc = make_desc(smem_u32(smem_v), UNIT * 128, 1024);
-        uint32_t q_phase = 0, p_phase = 0; // a bit per tile; per tile and place
-        uint32_t tile_i = 0, seg_i = 0;
+        const int t = warp - MMA_WARP; // 0, 1: the tile
+        uint32_t q_phase = 0, p_phase = 0, tile_i = 0, seg_i = 0; // p_phase: a bit per place
         bool ok = true;
-        auto scores = [&](int t, int st, int place) { // S_t = Q_t K^T, the place's half of a unit
+        auto scores = [&](int st, int place) { // S_t = Q_t K^T, the place's half of a unit
             const uint64_t a = q_desc + (uint64_t)(t * (S::MAT >> 4)), b = k_desc + (uint64_t)((st * S::MAT + place * STEP * 128) >> 4);
             if (elect_one()) {
 #pragma unroll
@@ -750,7 +752,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 tc_commit(&ctrl->s_full[t][place]);
             }
         };
-        auto weigh = [&](int t, int st, int place, bool more) { // O_t += P_t V
+        auto weigh = [&](int st, int place, bool more) { // O_t += P_t V
             const uint64_t b = v_desc + (uint64_t)((st * S::MAT + place * STEP * 128) >> 4);
             if (elect_one()) {
 #pragma unroll
@@ -765,45 +767,50 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         auto commit = [&](uint64_t *bar) {
             if (elect_one()) tc_commit(bar);
         };
-        while (warp == MMA_WARP && ok) {
+        while (t < 2 && ok) {
             const segment_t *seg = take(seg_i);
             if (!seg || seg->rows == 0) break;
             const int n = steps_of(*seg), units = seg->u1 - seg->u0;
-            const bool two = seg->rows > TILE;
+            const bool active = seg->rows > t * TILE;
             give_back(seg_i++);
             auto stage = [&](int s) { return (int)((tile_i + s / STEPS) % STAGES); };
             auto use = [&](int s) { return (tile_i + s / STEPS) / STAGES & 1; };
-            if (!(ok = warp_wait(&ctrl->k_full[stage(0)], use(0), ctrl, status))) break;
-            for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
-                if (!(ok = warp_wait(&ctrl->q_full[t], q_phase >> t & 1, ctrl, status))) break;
-                q_phase ^= 1u << t;
-                tc_fence_after();
-                scores(t, stage(0), 0);
-                if (n > 1) scores(t, stage(0), 1);
+            auto wait = [&](uint64_t *bar, uint32_t parity) { return ok = warp_wait(bar, parity, ctrl, status); };
+            if (!active) { // no rows in this tile: the stages are given back as they come
+                for (int s = 0; s < n; s += STEPS) {
+                    if (!wait(&ctrl->k_full[stage(s)], use(s))) break;
+                    if (lane == 0) mbar_arrive(&ctrl->k_empty[stage(s)]);
+                    if (!wait(&ctrl->v_full[stage(s)], use(s))) break;
+                    if (lane == 0) mbar_arrive(&ctrl->v_empty[stage(s)]);
+                }
+                tile_i += (uint32_t)units;
+                continue;
             }
-            if (!ok) break;
+            if (!wait(&ctrl->k_full[stage(0)], use(0)) || !wait(&ctrl->q_full[t], q_phase)) break;
+            q_phase ^= 1;
+            tc_fence_after();
+            scores(stage(0), 0);
+            if (n > 1) scores(stage(0), 1);
             commit(&ctrl->k_empty[stage(0)]);
             for (int s = 0; s < n; ++s) {
                 const int place = s % STEPS;
                 if (place == 0) {
-                    if (!(ok = warp_wait(&ctrl->v_full[stage(s)], use(s), ctrl, status))) break;
-                    if (s + 2 < n && !(ok = warp_wait(&ctrl->k_full[stage(s + 2)], use(s + 2), ctrl, status))) break;
+                    if (!wait(&ctrl->v_full[stage(s)], use(s))) break;
+                    if (s + 2 < n && !wait(&ctrl->k_full[stage(s + 2)], use(s + 2))) break;
                 }
-                for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
-                    const int bit = t * STEPS + place;
-                    if (!(ok = warp_wait(&ctrl->p_full[t][place], p_phase >> bit & 1, ctrl, status))) break;
-                    p_phase ^= 1u << bit;
-                    tc_fence_after();
-                    weigh(t, stage(s), place, s > 0);
-                    if (s + 2 < n) scores(t, stage(s + 2), place);
-                }
-                if (!ok) break;
+                if (!wait(&ctrl->p_full[t][place], p_phase >> place & 1)) break;
+                p_phase ^= 1u << place;
+                tc_fence_after();
+                weigh(stage(s), place, s > 0);
                 if (place == 1 || s + 1 == n) commit(&ctrl->v_empty[stage(s)]);
-                if (s + 2 < n && (place == 1 || s + 3 == n)) commit(&ctrl->k_empty[stage(s + 2)]);
+                if (s + 2 < n) {
+                    scores(stage(s + 2), place);
+                    if (place == 1 || s + 3 == n) commit(&ctrl->k_empty[stage(s + 2)]);
+                }
             }
             tile_i += (uint32_t)units;
         }
-        if (warp == MMA_WARP + 1) {
+        if (t == 2) {
             // ---------------- the segments ----------------
             int64_t at = line.begin;
             for (uint32_t i = 0;; ++i) {
