@@ -27,6 +27,7 @@ namespace kv_mma {
 
 using namespace kv_line;
 
+constexpr int EXTRA = 1; // units that an item's queries and result take besides
 constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32;
 static_assert(WARPS * STEP == UNIT, "a warp takes one step of each unit");
 
@@ -120,7 +121,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     const b200_kv_cache_t &c = p.cache;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     part_t line;
-    if (!begin_part<ROWS>(p, line, line_words)) return;
+    if (!begin_part<ROWS, EXTRA>(p, line, line_words)) return;
     const int heads = line.heads, group = line.group, page = (int)c.page, pieces = (int)c.dim / 16;
     uint8_t *ring = smem + warp * S::RING;
     uint2 *q_shared = (uint2 *)(smem + WARPS * S::RING);
@@ -135,11 +136,13 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     constexpr size_t part_size = (size_t)ROWS * (DP + 2); // part_floats()
     int64_t at = line.begin;
     while (at < line.stop) {
-        const place_t place_at = find_item<ROWS>(p, line, at);
+        const place_t place_at = find_item<ROWS, EXTRA>(p, line, at);
+        at = place_at.next;
+        const int u0 = place_at.u0, u1 = place_at.u1;
+        if (u1 <= u0) continue; // none of its tokens
         const item_t item = place_at.item;
         const int head = place_at.head, tile = place_at.tile, seq = line.seq;
         const seq_t s = line.s;
-        const int u0 = (int)(at - place_at.item_begin), u1 = (int)min((int64_t)item.units, line.stop - place_at.item_begin);
         const int rows = (s.end - s.begin) * group - tile * ROWS; // that exist from here on
         const int end = min(u1 * UNIT, item.tokens);
         if (tid == 0 && u0 == 0 && (int64_t)s.first + (s.end - s.begin) > line.capacity) flag_bad_page(c);
@@ -510,8 +513,8 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             }
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == item.units;
-        float *part = parts + (size_t)(blockIdx.x * 2 + (at == line.begin ? 0 : 1)) * part_size;
+        const bool whole = place_at.whole();
+        float *part = parts + place_at.part(blockIdx.x) * part_size;
         const int live = min(rows, ROWS);
         for (int i = tid; i < live * (DP / 4); i += THREADS) {
             const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
@@ -544,7 +547,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
 
         // ---- an item in several parts: the last block to finish one puts them together
         if (!whole) {
-            const int c0 = owner(line, place_at.item_begin), c1 = owner(line, place_at.item_begin + item.units - 1);
+            const int c0 = place_at.c0, c1 = place_at.c1;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -555,7 +558,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             __syncthreads();
             if (last_part) {
                 __threadfence();
-                auto part_of = [&](int b) { return parts + part_index(line, place_at.item_begin, c0, b) * part_size; };
+                auto part_of = [&](int b) { return parts + place_at.part(b) * part_size; };
                 // the parts' weights into shared memory: factor = 2^(m - largest m), then the values eight parts at a time
                 const int n = c1 - c0 + 1;
                 float *fs = (float *)smem; // [n][ROWS]; the host keeps the grid small enough
@@ -611,7 +614,6 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             for (int i = tid; i < WARPS * S::RING / 16; i += THREADS) ((uint4 *)smem)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
         }
-        at = place_at.item_begin + u1;
     }
 }
 

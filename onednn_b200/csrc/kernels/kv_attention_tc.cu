@@ -38,6 +38,7 @@ constexpr int SOFTMAX_WARPS = 8, CONVERT_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + C
 // registers per thread: what the launch gives every warp, and how the four groups of four warps share it
 constexpr int REGS = 128, SOFTMAX_REGS = 176, CONVERT_REGS = 104, MMA_REGS = 56;
 static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * REGS && THREADS * REGS <= 65536, "");
+constexpr int EXTRA = 3;   // units that an item's queries, filling and draining, and result take besides (8 of 2.5 us)
 constexpr int STAGES = 2;  // of keys and of values
 constexpr int CHUNKS = UNIT / 16;
 constexpr int STEP = 64, STEPS = UNIT / STEP; // tokens of a step; steps of a unit, which the converters work on
@@ -68,11 +69,9 @@ struct segment_t {
     int row0, first;   // the item's first query row in the sequence; token of the sequence's first row
     int head, seq;
     int tokens;        // that the item's last row sees
-    int u0, u1;        // units, of
-    int units;
+    int u0, u1;        // units
+    int whole;         // all of the item's
     int c0, c1;        // the blocks that share the item
-    int slot;          // where its partial result goes
-    int parity;        // which of block c0's two partial results is the item's
     int over;          // whether the sequence has tokens beyond the table
 };
 constexpr int SEGMENTS = 4;
@@ -272,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     uint32_t *status = c.status;
 
     part_t line;
-    if (!begin_part<ROWS>(p, line, ctrl->line_words)) return;
+    if (!begin_part<ROWS, EXTRA>(p, line, ctrl->line_words)) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctrl->q_full[i], SOFTMAX_WARPS / 2);
@@ -338,17 +337,22 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             join_phase ^= 1;
             return ok;
         };
-        // this thread's query row of a segment, as it is, into its place in shared memory
+        // the warp's query rows of a segment, as they are, into their places in shared memory; a row by DP / 8 lanes
         auto fetch = [&](const segment_t &g) {
+            int64_t at = -1;
             if (t * TILE + r < g.rows) {
                 const int idx = g.row0 + t * TILE + r;
-                const char *from = (const char *)p.query
-                        + ((int64_t)(g.begin + idx / group) * p.query_s0 + ((int64_t)g.head * group + idx % group) * p.query_s1) * 2;
+                at = (int64_t)(g.begin + idx / group) * p.query_s0 + ((int64_t)g.head * group + idx % group) * p.query_s1;
+            }
+            constexpr int PIECES = DP / 8;
 #pragma unroll
-                for (int i = 0; i < DP / 8; ++i)
-                    if (i * 8 < c.dim)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_q + t * S::MAT + piece_at(r, i))), "l"(from + i * 16)
-                                     : "memory");
+            for (int i = 0; i < PIECES; ++i) {
+                const int row = i * (32 / PIECES) + lane / PIECES, piece = lane % PIECES;
+                const int64_t from = __shfl_sync(~0u, at, row);
+                if (from >= 0 && piece * 8 < c.dim)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_q + t * S::MAT + piece_at((warp & 3) * 32 + row, piece))),
+                                 "l"((const char *)p.query + (from + piece * 8) * 2)
+                                 : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -356,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         // A negative softmax scale turns the query round, so that factors of the scores are positive.
         auto prepare = [&](bool there) {
             asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
             uint8_t *to = smem_q + t * S::MAT;
             uint32_t top2 = 0; // the largest magnitudes' bits, of even and of odd elements
 #pragma unroll 4
@@ -519,11 +524,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             tile_i += (uint32_t)(u1 - u0);
 
             // ---- the row's result, or its part of it
-            const bool whole = u0 == 0 && u1 == seg->units;
+            const bool whole = seg->whole;
             if (l != l) m = INFINITY; // a NaN among the scores, which no maximum shows
             const int idx = seg->row0 + t * TILE + r;
             char *to = (char *)p.dst + ((int64_t)(seg->begin + idx / group) * p.dst_s0 + ((int64_t)seg->head * group + idx % group) * p.dst_s1) * 2;
-            float *part = parts + (size_t)(blockIdx.x * 2 + seg->slot) * part_size;
+            auto part_of = [&](int b) { return parts + ((size_t)b * 2 + (b == seg->c0 ? 1 : 0)) * part_size; }; // place_t::part
+            float *part = part_of(blockIdx.x);
             const int pr = t * TILE + r; // row of the item
             auto put = [&](int d, const float (&x)[8], float inv) { // eight dims of the result
                 if (d >= c.dim) return;
@@ -568,7 +574,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 }
                 if (ok && join() && ctrl->last_part && mine) {
                     __threadfence();
-                    auto part_of = [&](int b) { return parts + ((size_t)b * 2 + (b == c0 ? seg->parity : 0)) * part_size; };
                     float mm = -INFINITY, ll = 0.f;
 #pragma unroll 4
                     for (int b = c0; b <= c1; ++b) mm = fmaxf(mm, __ldcg(part_of(b) + pr));
@@ -816,9 +821,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             for (uint32_t i = 0;; ++i) {
                 segment_t g;
                 g.rows = 0;
-                const bool more = at < line.stop;
-                if (more) {
-                    const place_t q = find_item<ROWS>(p, line, at);
+                while (at < line.stop && g.rows == 0) {
+                    const place_t q = find_item<ROWS, EXTRA>(p, line, at);
+                    at = q.next;
+                    if (q.u1 <= q.u0) continue; // the block has none of its tokens
                     g.begin = line.s.begin;
                     g.row0 = q.tile * ROWS;
                     g.rows = (line.s.end - line.s.begin) * group - g.row0;
@@ -826,16 +832,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     g.head = q.head;
                     g.seq = line.seq;
                     g.tokens = q.item.tokens;
-                    g.u0 = (int)(at - q.item_begin);
-                    g.u1 = (int)min((int64_t)q.item.units, line.stop - q.item_begin);
-                    g.units = q.item.units;
-                    g.c0 = owner(line, q.item_begin);
-                    g.c1 = owner(line, q.item_begin + q.item.units - 1);
-                    g.slot = at == line.begin ? 0 : 1;
-                    g.parity = (int)(part_index(line, q.item_begin, g.c0, g.c0) & 1);
+                    g.u0 = q.u0;
+                    g.u1 = q.u1;
+                    g.whole = q.whole();
+                    g.c0 = q.c0;
+                    g.c1 = q.c1;
                     g.over = (int64_t)line.s.first + (line.s.end - line.s.begin) > line.capacity;
-                    at = q.item_begin + g.u1;
                 }
+                const bool more = g.rows > 0;
                 if (i >= SEGMENTS && !warp_wait(&ctrl->seg_empty[i % SEGMENTS], (i / SEGMENTS - 1) & 1, ctrl, status)) break;
                 if (lane == 0) {
                     ctrl->segments[i % SEGMENTS] = g;

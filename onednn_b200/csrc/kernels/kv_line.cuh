@@ -1,8 +1,9 @@
 // How the attention kernels divide a ragged batch among the SMs.
 //
 // An item is one sequence, one key head and ROWS query rows (tokens x the query heads of the key head); it costs its
-// tokens, in units of 128.  All items side by side -- sequence, head, rows -- form one line of units, which is cut into
-// equal parts, one per block, wherever that falls.  The host knows neither offsets nor lengths, so every
+// tokens, in units of 128, and EXTRA units for what its beginning and end take.  All items side by side -- sequence,
+// head, rows -- form one line of units, which is cut into equal parts, one per block, wherever that falls (a part that
+// ends within the extra units has no token of that item).  The host knows neither offsets nor lengths, so every
 // block derives the line itself, in two short scans over the sequences.
 #pragma once
 
@@ -31,11 +32,11 @@ __device__ __forceinline__ item_t item_of(const seq_t &s, int group, int tile, i
 }
 
 // units of one key head of a sequence, the lanes of a warp side by side
-template <int ROWS>
+template <int ROWS, int EXTRA>
 __device__ __forceinline__ int64_t head_units_warp(const seq_t &s, int group, int64_t capacity) {
     const int tiles = ((s.end - s.begin) * group + ROWS - 1) / ROWS;
     int64_t n = 0;
-    for (int tile = threadIdx.x & 31; tile < tiles; tile += 32) n += item_of<ROWS>(s, group, tile, capacity).units;
+    for (int tile = threadIdx.x & 31; tile < tiles; tile += 32) n += item_of<ROWS>(s, group, tile, capacity).units + EXTRA;
 #pragma unroll
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
     return n;
@@ -43,19 +44,19 @@ __device__ __forceinline__ int64_t head_units_warp(const seq_t &s, int group, in
 
 // the same for a sequence of its own per lane (`there`: the lane has one): short ones by their lanes, the others by the
 // whole warp, one after the other
-template <int ROWS>
+template <int ROWS, int EXTRA>
 __device__ __forceinline__ int64_t head_units_lanes(const seq_t &s, bool there, int group, int64_t capacity) {
     const int tiles = there ? ((s.end - s.begin) * group + ROWS - 1) / ROWS : 0;
     int64_t n = 0;
     if (tiles <= 4)
-        for (int tile = 0; tile < tiles; ++tile) n += item_of<ROWS>(s, group, tile, capacity).units;
+        for (int tile = 0; tile < tiles; ++tile) n += item_of<ROWS>(s, group, tile, capacity).units + EXTRA;
     for (uint32_t todo = __ballot_sync(~0u, tiles > 4); todo; todo &= todo - 1) {
         const int k = __ffs(todo) - 1;
         seq_t one;
         one.begin = __shfl_sync(~0u, s.begin, k);
         one.end = __shfl_sync(~0u, s.end, k);
         one.first = __shfl_sync(~0u, s.first, k);
-        const int64_t m = head_units_warp<ROWS>(one, group, capacity);
+        const int64_t m = head_units_warp<ROWS, EXTRA>(one, group, capacity);
         if ((int)(threadIdx.x & 31) == k) n = m;
     }
     return n;
@@ -91,11 +92,18 @@ struct part_t {
 struct place_t {
     int head, tile;
     item_t item;
-    int64_t item_begin;
+    int64_t item_begin; // on the line
+    int u0, u1;         // the item's units of tokens that the block has, none when u1 <= u0
+    int64_t next;       // where it goes on
+    int c0, c1;         // the blocks that share the item
+
+    __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == item.units; }
+    // a block has two places for partial results: [0] of the item that it begins in, [1] of the one that it ends in
+    __device__ __forceinline__ size_t part(int b) const { return (size_t)b * 2 + (b == c0 ? 1 : 0); }
 };
 
 // All threads of the block.  False: the block has no part.  `shared`: 34 words that nothing else uses meanwhile.
-template <int ROWS>
+template <int ROWS, int EXTRA>
 __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, part_t &l, int64_t *shared) {
     const b200_kv_cache_t &c = p.cache;
     const int tid = threadIdx.x, threads = blockDim.x;
@@ -108,7 +116,7 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
         const int b = base + tid;
         seq_t s = {0, 0, 0};
         if (b < c.seqs) s = load_seq(c, b, p.rows);
-        int64_t n = head_units_lanes<ROWS>(s, b < c.seqs, l.group, l.capacity) * l.heads;
+        int64_t n = head_units_lanes<ROWS, EXTRA>(s, b < c.seqs, l.group, l.capacity) * l.heads;
         n = block_scan(n, warp_sum);
         if (tid == threads - 1) words[0] = n;
         __syncthreads();
@@ -125,7 +133,7 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
         const int b = base + tid;
         seq_t s = {0, 0, 0};
         if (b < c.seqs) s = load_seq(c, b, p.rows);
-        const int64_t n = head_units_lanes<ROWS>(s, b < c.seqs, l.group, l.capacity) * l.heads;
+        const int64_t n = head_units_lanes<ROWS, EXTRA>(s, b < c.seqs, l.group, l.capacity) * l.heads;
         const int64_t upto = l.seq_begin + block_scan(n, warp_sum);
         __syncthreads();
         if (tid == 0) words[0] = -1;
@@ -142,17 +150,36 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
         __syncthreads();
     }
     l.s = load_seq(c, l.seq, p.rows);
-    l.per_head = head_units_warp<ROWS>(l.s, l.group, l.capacity);
+    l.per_head = head_units_warp<ROWS, EXTRA>(l.s, l.group, l.capacity);
     return true;
 }
 
+// the block whose part holds unit u
+__device__ __forceinline__ int owner(const part_t &l, int64_t u) {
+    int64_t o = u * l.blocks / l.total;
+    while (l.total * (o + 1) / l.blocks <= u) ++o;
+    while (l.total * o / l.blocks > u) --o;
+    return (int)o;
+}
+
+// what the block has of an item, and who has the rest
+template <int EXTRA>
+__device__ __forceinline__ void cut(const part_t &l, int64_t at, place_t &q) {
+    const int64_t tokens = q.item_begin + EXTRA; // where the item's tokens begin on the line
+    q.u0 = (int)max((int64_t)0, at - tokens);
+    q.u1 = (int)min((int64_t)q.item.units, l.stop - tokens);
+    q.next = tokens + q.item.units;
+    q.c0 = owner(l, tokens);
+    q.c1 = owner(l, tokens + q.item.units - 1);
+}
+
 // the item at unit `at`, which never goes back; whole warps
-template <int ROWS>
+template <int ROWS, int EXTRA>
 __device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p, part_t &l, int64_t at) {
     while (at - l.seq_begin >= l.per_head * l.heads) {
         l.seq_begin += l.per_head * l.heads;
         l.s = load_seq(p.cache, ++l.seq, p.rows);
-        l.per_head = head_units_warp<ROWS>(l.s, l.group, l.capacity);
+        l.per_head = head_units_warp<ROWS, EXTRA>(l.s, l.group, l.capacity);
     }
     place_t q;
     q.head = (int)((at - l.seq_begin) / l.per_head);
@@ -161,15 +188,16 @@ __device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p
     q.tile = 0;
     if ((l.s.end - l.s.begin) * l.group <= 4 * ROWS) { // few items: one after the other
         q.item = item_of<ROWS>(l.s, l.group, 0, l.capacity);
-        while (at - q.item_begin >= q.item.units) {
-            q.item_begin += q.item.units;
+        while (at - q.item_begin >= q.item.units + EXTRA) {
+            q.item_begin += q.item.units + EXTRA;
             q.item = item_of<ROWS>(l.s, l.group, ++q.tile, l.capacity);
         }
+        cut<EXTRA>(l, at, q);
         return q;
     }
     for (;; q.tile += 32) { // 32 items at a time
         const item_t mine = item_of<ROWS>(l.s, l.group, q.tile + lane, l.capacity);
-        int64_t upto = mine.units;
+        int64_t upto = mine.units ? mine.units + EXTRA : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t u = __shfl_up_sync(~0u, upto, o);
@@ -181,29 +209,17 @@ __device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p
             q.tile += k;
             q.item.tokens = __shfl_sync(~0u, mine.tokens, k);
             q.item.units = __shfl_sync(~0u, mine.units, k);
-            q.item_begin += __shfl_sync(~0u, upto, k) - q.item.units;
+            q.item_begin += __shfl_sync(~0u, upto, k) - q.item.units - EXTRA;
+            cut<EXTRA>(l, at, q);
             return q;
         }
         q.item_begin += __shfl_sync(~0u, upto, 31);
     }
 }
 
-// the block whose part holds unit u
-__device__ __forceinline__ int owner(const part_t &l, int64_t u) {
-    int64_t o = u * l.blocks / l.total;
-    while (l.total * (o + 1) / l.blocks <= u) ++o;
-    while (l.total * o / l.blocks > u) --o;
-    return (int)o;
-}
-
 // Scratch: a counter per block (parts done of the item that begins in its stretch of the line and ends in another's;
-// zero between launches), then per block two partial results: [0] of the item that it begins in, [1] of the one it ends in.
+// zero between launches), then per block two partial results.
 __host__ __device__ inline size_t counter_bytes(int blocks) { return ((size_t)blocks * 4 + 255) / 256 * 256; }
-
-// the partial result of block b, one of those that share the item from `item_begin` on
-__device__ __forceinline__ size_t part_index(const part_t &l, int64_t item_begin, int first, int b) {
-    return (size_t)b * 2 + (b == first && l.total * b / l.blocks != item_begin ? 1 : 0);
-}
 
 } // namespace kv_line
 } // namespace b200
