@@ -32,7 +32,7 @@ constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32;
 static_assert(WARPS * STEP == UNIT, "a warp takes one step of each unit");
 
 // blocks per SM
-__host__ __device__ constexpr int blocks_of(int dp, int nb) { return dp == 64 ? (nb == 1 ? 4 : nb == 2 ? 3 : 2) : dp == 128 ? (nb == 1 ? 3 : 2) : 1; }
+__host__ __device__ constexpr int blocks_of(int dp, int nb) { return dp == 64 ? (nb == 1 ? 4 : 3) : dp == 128 ? (nb == 1 ? 3 : 2) : 1; }
 
 template <int DP, int NB>
 struct shape_t {
