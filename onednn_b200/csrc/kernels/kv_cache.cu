@@ -15,6 +15,19 @@ __device__ __forceinline__ float finite_abs(float x) {
 }
 __device__ __forceinline__ float no_nan(float x) { return x == x ? x : 0.f; }
 
+// magnitudes' bits of eight 16-bit values against the largest so far, even and odd elements side by side
+__device__ __forceinline__ uint32_t top_bits(uint32_t top, const uint4 &u) {
+    return __vmaxu2(__vmaxu2(top, u.x & 0x7fff7fffu), __vmaxu2(__vmaxu2(u.y & 0x7fff7fffu, u.z & 0x7fff7fffu), u.w & 0x7fff7fffu));
+}
+__device__ __forceinline__ void widen8(bool bf16, const uint4 &u, float (&v)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = bf16 ? bf16x2_to_f32(w[i]) : f16x2_to_f32(w[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+
 // The new tokens of one sequence in one page, one head: the largest magnitude, the page's scale,
 // the codes.  All threads of the block, and no two blocks on the same page and head.
 template <bool VEC>
@@ -25,7 +38,27 @@ __device__ __forceinline__ void append_page(const b200_kv_rows_params_t &p, cons
     const int unit = VEC ? 8 : 1, per = dim / unit, esize = dt_bits(p.dt) / 8;
     const char *rows = src + row * p.s_row * esize;
     float top = 0.f;
-    for (int i = tid; i < count * per; i += APPEND_THREADS) {
+    // 16-bit rows of up to KEEP accesses per thread stay in registers between the two passes, as long as all values are finite
+    constexpr int KEEP = VEC ? 8 : 1;
+    uint4 kept[KEEP];
+    bool keep = VEC && p.dt != B200_DT_F32 && count * per <= KEEP * APPEND_THREADS;
+    const bool bf16 = p.dt == B200_DT_BF16;
+    if (keep) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+            const int i = k * APPEND_THREADS + tid, r = i / per;
+            kept[k] = make_uint4(0, 0, 0, 0);
+            if (i < count * per) kept[k] = *(const uint4 *)(rows + (r * p.s_row + (i - r * per) * 8) * 2);
+        }
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) bits = top_bits(bits, kept[k]);
+        const float2 f = bf16 ? bf16x2_to_f32(bits) : f16x2_to_f32(bits);
+        top = fmaxf(f.x, f.y);
+        keep = !__syncthreads_or(!(f.x < INFINITY && f.y < INFINITY)); // an infinity or NaN does not count: value by value, below
+        if (!keep) top = 0.f;
+    }
+    for (int i = keep ? count * per : tid; i < count * per; i += APPEND_THREADS) {
         const int r = i / per, e = (i - r * per) * unit;
         const char *at = rows + (r * p.s_row + e) * esize;
         if (VEC) {
@@ -66,7 +99,19 @@ __device__ __forceinline__ void append_page(const b200_kv_rows_params_t &p, cons
         }
     }
     codes += (int64_t)slot * c.s_slot;
-    for (int i = tid; i < count * per; i += APPEND_THREADS) {
+    if (keep) {
+#pragma unroll
+        for (int k = 0; k < KEEP; ++k) {
+            const int i = k * APPEND_THREADS + tid, r = i / per;
+            if (i >= count * per) break;
+            float v[8];
+            widen8(bf16, kept[k], v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= inv;
+            *(uint2 *)(codes + r * c.s_slot + (i - r * per) * 8) = make_uint2(codes4(c.dt, v[0], v[1], v[2], v[3]), codes4(c.dt, v[4], v[5], v[6], v[7]));
+        }
+    }
+    for (int i = keep ? count * per : tid; i < count * per; i += APPEND_THREADS) {
         const int r = i / per, e = (i - r * per) * unit;
         const char *at = rows + (r * p.s_row + e) * esize;
         uint8_t *d = codes + r * c.s_slot + e;
@@ -74,10 +119,10 @@ __device__ __forceinline__ void append_page(const b200_kv_rows_params_t &p, cons
             float v[8];
             load8(p.dt, at, v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = no_nan(v[j]) * inv;
+            for (int j = 0; j < 8; ++j) v[j] = held(c.dt, no_nan(v[j]) * inv);
             *(uint2 *)d = make_uint2(codes4(c.dt, v[0], v[1], v[2], v[3]), codes4(c.dt, v[4], v[5], v[6], v[7]));
         } else {
-            *d = code1(c.dt, no_nan(load_f32(p.dt, at, 0)) * inv);
+            *d = code1(c.dt, held(c.dt, no_nan(load_f32(p.dt, at, 0)) * inv));
         }
     }
     __syncthreads(); // `part` is free again
@@ -138,25 +183,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(const __grid_
     }
 }
 
-// One warp per row: keys and values of all heads of one token.
 template <bool VEC>
-__global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ b200_kv_rows_params_t p) {
+__device__ __forceinline__ void read_row(const b200_kv_rows_params_t &p, const seq_t &s, int b, int64_t row, int lane) {
     const b200_kv_cache_t &c = p.cache;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= p.rows) return;
-    int b = -1;
-    for (int base = 0; base < c.seqs; base += 32) {
-        const int i = base + lane;
-        const bool in = i < c.seqs && c.offsets[i] <= row && row < c.offsets[i + 1];
-        const uint32_t m = __ballot_sync(~0u, in);
-        if (m) {
-            b = base + __ffs(m) - 1;
-            break;
-        }
-    }
-    if (b < 0) return;
-    const seq_t s = load_seq(c, b, p.rows);
     const int at = s.first + (int)(row - s.begin);
     int slot = 0, phys = -1;
     if (at >= 0) {
@@ -165,27 +194,44 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ b2
     }
     const int unit = VEC ? 16 : 1, per = (int)c.dim / unit, all = per * (int)c.heads, esize = dt_bits(p.dt) / 8;
     const int64_t place = (int64_t)phys * c.s_page + (int64_t)slot * c.s_slot;
+    auto put = [&](char *d, const uint4 &w, float scale) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float a[4], bb[4], v[8];
+            code_values4(c.dt, u[2 * j], a);
+            code_values4(c.dt, u[2 * j + 1], bb);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t] = a[t] * scale, v[4 + t] = bb[t] * scale;
+            store8(p.dt, d + 8 * j * esize, v);
+        }
+    };
     for (int i = lane; i < 2 * all; i += 32) {
         const bool val = i >= all;
         const int k = val ? i - all : i, head = k / per, e = (k - head * per) * unit;
         char *d = (char *)(val ? p.value : p.key) + (row * p.s_row + head * p.s_head + e) * esize;
         const uint8_t *from = (const uint8_t *)(val ? c.value : c.key) + place + head * c.s_head + e;
         const float scale = phys < 0 ? 0.f : (val ? c.value_scale : c.key_scale)[(int64_t)phys * c.heads + head];
-        if (VEC) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (phys >= 0) w = *(const uint4 *)from;
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float a[4], bb[4], v[8];
-                code_values4(c.dt, u[2 * j], a);
-                code_values4(c.dt, u[2 * j + 1], bb);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) v[t] = a[t] * scale, v[4 + t] = bb[t] * scale;
-                store8(p.dt, d + 8 * j * esize, v);
-            }
-        } else {
-            store1(p.dt, d, 0, phys < 0 ? 0.f : code_value(c.dt, *from) * scale);
+        if (VEC) put(d, phys < 0 ? make_uint4(0, 0, 0, 0) : *(const uint4 *)from, scale);
+        else store1(p.dt, d, 0, phys < 0 ? 0.f : code_value(c.dt, *from) * scale);
+    }
+}
+
+// One warp per row: keys and values of all heads of one token.
+template <bool VEC>
+__global__ void __launch_bounds__(128) kv_read_kernel(const __grid_constant__ b200_kv_rows_params_t p) {
+    const b200_kv_cache_t &c = p.cache;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= p.rows) return;
+    for (int base = 0; base < c.seqs; base += 32) {
+        const int i = base + lane;
+        const bool in = i < c.seqs && c.offsets[i] <= row && row < c.offsets[i + 1];
+        const uint32_t m = __ballot_sync(~0u, in);
+        if (m) {
+            const int b = base + __ffs(m) - 1;
+            read_row<VEC>(p, load_seq(c, b, p.rows), b, row, lane);
+            return;
         }
     }
 }

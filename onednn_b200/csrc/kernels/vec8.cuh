@@ -71,9 +71,13 @@ __device__ __forceinline__ float code_peak_factor(int dt) { return dt == B200_DT
 // values next to them) need no special case
 constexpr float CODE_SCALE_MIN = 1.17549435e-38f; // 2^-126
 
-__device__ __forceinline__ uint32_t code_s8(float v) {
-    v = v < -127.f ? -127.f : v; // NaN passes and converts to 0
-    return cvt_sat_s8(v);
+// The caller's values lie within the peak already, up to a rounding (a row or page times the reciprocal of its own
+// scale; `held` below for the others).  s8: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the
+// low byte -- on the ordinary f32 pipe, where a conversion instruction runs at an eighth of the rate.
+__device__ __forceinline__ uint32_t round_s8(float v) { return __float_as_uint(__fadd_rn(v, 12582912.f)); }
+__device__ __forceinline__ float held(int dt, float v) { // to the peak; NaN is not for here
+    const float peak = dt == B200_DT_S8 ? 127.f : 448.f;
+    return fminf(fmaxf(v, -peak), peak);
 }
 // two values, the first in the low byte; rounded once, held to +-448, NaN is 0x7f
 __device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi) {
@@ -82,18 +86,20 @@ __device__ __forceinline__ uint32_t code_e4m3x2(float lo, float hi) {
     return r;
 }
 __device__ __forceinline__ uint32_t codes4(int dt, float a, float b, float c, float d) {
-    if (dt == B200_DT_S8) return code_s8(a) | code_s8(b) << 8 | code_s8(c) << 16 | code_s8(d) << 24;
+    if (dt == B200_DT_S8)
+        return __byte_perm(__byte_perm(round_s8(a), round_s8(b), 0x0040), __byte_perm(round_s8(c), round_s8(d), 0x0040), 0x5410);
     return code_e4m3x2(a, b) | code_e4m3x2(c, d) << 16;
 }
 __device__ __forceinline__ uint8_t code1(int dt, float v) {
-    return dt == B200_DT_S8 ? (uint8_t)code_s8(v) : (uint8_t)code_e4m3x2(v, 0.f);
+    return dt == B200_DT_S8 ? (uint8_t)round_s8(v) : (uint8_t)code_e4m3x2(v, 0.f);
 }
 __device__ __forceinline__ float code_value(int dt, uint8_t c) { return dt == B200_DT_S8 ? (float)(int8_t)c : e4m3_to_f32(c); }
 // the four codes of a word
 __device__ __forceinline__ void code_values4(int dt, uint32_t w, float (&v)[4]) {
     if (dt == B200_DT_S8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> (8 * i));
+        for (int i = 0; i < 4; ++i) // code + 128 in the low byte of 2^23, minus 2^23 + 128: exact
+            v[i] = __uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4b000000u, 0x7540 + i)) - 8388736.f;
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
