@@ -114,7 +114,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     using S = shape_t<DP, NB>;
     constexpr int ROWS = S::ROWS, KS = DP / 16, CH = DP / 16, MT = DP / 16;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t line_words[34];
+    __shared__ int64_t line_words[LINE_WORDS];
     __shared__ float merge_m[WARPS][ROWS], merge_l[WARPS][ROWS];
     __shared__ bool last_part;
 

@@ -85,7 +85,7 @@ struct ctrl_t {
     volatile uint32_t abort;
     uint32_t last_part;
     scales_t scales[4];
-    int64_t line_words[34];
+    int64_t line_words[LINE_WORDS];
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -13,6 +13,7 @@ namespace b200 {
 namespace kv_line {
 
 constexpr int UNIT = 128;
+constexpr int LINE_WORDS = 35;
 
 struct item_t {
     int tokens; // that its last row sees
@@ -80,7 +81,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sum) {
 // a block's part of the line, and the sequence that it stands in
 struct part_t {
     int64_t total, begin, stop;
-    int blocks; // that have a part: none is empty
+    int blocks; // that have a part; none is empty
     int group, heads;
     int64_t capacity; // tokens that a row of the table can hold
     int seq;
@@ -102,7 +103,7 @@ struct place_t {
     __device__ __forceinline__ size_t part(int b) const { return (size_t)b * 2 + (b == c0 ? 1 : 0); }
 };
 
-// All threads of the block.  False: the block has no part.  `shared`: 34 words that nothing else uses meanwhile.
+// All threads of the block.  False: the block has no part.  `shared`: LINE_WORDS words that nothing else uses meanwhile.
 template <int ROWS, int EXTRA>
 __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, part_t &l, int64_t *shared) {
     const b200_kv_cache_t &c = p.cache;
@@ -111,44 +112,43 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
     l.group = (int)(p.q_heads / c.heads);
     l.heads = (int)c.heads;
     l.capacity = min((int64_t)0x7fffff00, c.table_cols * c.page);
-    l.total = 0;
-    for (int base = 0; base < c.seqs; base += threads) {
+    // the units of `threads` sequences, one per thread, and of all up to this one
+    int64_t n = 0, upto = 0;
+    auto scan = [&](int base) {
         const int b = base + tid;
         seq_t s = {0, 0, 0};
         if (b < c.seqs) s = load_seq(c, b, p.rows);
-        int64_t n = head_units_lanes<ROWS, EXTRA>(s, b < c.seqs, l.group, l.capacity) * l.heads;
-        n = block_scan(n, warp_sum);
-        if (tid == threads - 1) words[0] = n;
+        n = head_units_lanes<ROWS, EXTRA>(s, b < c.seqs, l.group, l.capacity) * l.heads;
+        upto = block_scan(n, warp_sum);
+        if (tid == threads - 1) words[2] = upto;
+        if (tid == 0) words[0] = -1;
         __syncthreads();
-        l.total += words[0];
-    }
+        return words[2];
+    };
+    l.total = 0;
+    for (int base = 0; base < c.seqs; base += threads) l.total += scan(base);
+    // As many parts as units, if there are blocks for them: parts of at least two or four units were slower (four short
+    // sequences 14 and 16 us instead of 12), the joining costs less than a second unit.
     l.blocks = (int)min((int64_t)gridDim.x, l.total);
     if (blockIdx.x >= l.blocks) return false;
     l.begin = l.total * blockIdx.x / l.blocks;
     l.stop = l.total * (blockIdx.x + 1) / l.blocks;
     // the sequence that the part begins in, and the units before it
-    l.seq = 0;
     l.seq_begin = 0;
     for (int base = 0; base < c.seqs; base += threads) {
-        const int b = base + tid;
-        seq_t s = {0, 0, 0};
-        if (b < c.seqs) s = load_seq(c, b, p.rows);
-        const int64_t n = head_units_lanes<ROWS, EXTRA>(s, b < c.seqs, l.group, l.capacity) * l.heads;
-        const int64_t upto = l.seq_begin + block_scan(n, warp_sum);
-        __syncthreads();
-        if (tid == 0) words[0] = -1;
-        __syncthreads();
-        if (upto > l.begin && upto - n <= l.begin) words[0] = b, words[1] = upto - n;
-        if (tid == threads - 1) warp_sum[0] = upto;
-        __syncthreads();
-        if (words[0] >= 0) {
-            l.seq = (int)words[0];
-            l.seq_begin = words[1];
-            break;
+        int64_t sum = words[2];
+        if (c.seqs > threads) { // else the one scan has it
+            __syncthreads();
+            sum = scan(base);
         }
-        l.seq_begin = warp_sum[0];
+        if (l.seq_begin + upto > l.begin && l.seq_begin + upto - n <= l.begin) words[0] = base + tid, words[1] = l.seq_begin + upto - n;
         __syncthreads();
+        if (words[0] >= 0) break;
+        l.seq_begin += sum;
     }
+    if (words[0] < 0) return false; // the lengths changed under the kernel
+    l.seq = (int)words[0];
+    l.seq_begin = words[1];
     l.s = load_seq(c, l.seq, p.rows);
     l.per_head = head_units_warp<ROWS, EXTRA>(l.s, l.group, l.capacity);
     return true;
@@ -176,12 +176,17 @@ __device__ __forceinline__ void cut(const part_t &l, int64_t at, place_t &q) {
 // the item at unit `at`, which never goes back; whole warps
 template <int ROWS, int EXTRA>
 __device__ __forceinline__ place_t find_item(const b200_kv_attention_params_t &p, part_t &l, int64_t at) {
+    place_t q;
     while (at - l.seq_begin >= l.per_head * l.heads) {
         l.seq_begin += l.per_head * l.heads;
-        l.s = load_seq(p.cache, ++l.seq, p.rows);
+        if (++l.seq >= p.cache.seqs) { // not unless the lengths changed under the kernel
+            q.u0 = q.u1 = 0;
+            q.next = l.stop;
+            return q;
+        }
+        l.s = load_seq(p.cache, l.seq, p.rows);
         l.per_head = head_units_warp<ROWS, EXTRA>(l.s, l.group, l.capacity);
     }
-    place_t q;
     q.head = (int)((at - l.seq_begin) / l.per_head);
     q.item_begin = l.seq_begin + q.head * l.per_head;
     const int lane = threadIdx.x & 31;
