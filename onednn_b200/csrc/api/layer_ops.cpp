@@ -105,7 +105,9 @@ dnnl_status_t check_cache(const dnnl_memory_desc &cache, const dnnl_memory_desc 
     if (cache.dims[1] < 1 || cache.dims[2] < 1 || cache.dims[3] < 1) return dnnl_invalid_arguments;
     // heads are a grid dimension of the kernels; positions in a sequence are s32
     if (cache.dims[1] > 65535 || table.dims[0] > (1 << 24)) return dnnl_unimplemented;
+    // the kernels count inside a page, and across the heads of a token, in 32 bits
     if (cache.dims[2] > (1 << 20) || cache.dims[3] > (1 << 20)) return dnnl_unimplemented;
+    if (cache.dims[2] * cache.dims[3] > (1 << 30) || cache.dims[1] * cache.dims[3] > (1 << 30)) return dnnl_unimplemented;
     if (cache.dims[0] > std::numeric_limits<int32_t>::max()) return dnnl_unimplemented; // pages are s32
     return dnnl_success;
 }
@@ -131,7 +133,7 @@ void *at(const std::map<int, dnnl_memory *> &args, int arg) {
 
 dnnl_status_t status_of(int rc) {
     if (rc == 0) return dnnl_success;
-    if (rc == B200_ERR_UNSUPPORTED) return dnnl_unimplemented;
+    if (rc == B200_ERR_UNSUPPORTED || rc == B200_ERR_TOO_LARGE) return dnnl_unimplemented;
     if (rc == B200_ERR_BAD_ARG) return dnnl_invalid_arguments;
     return dnnl_runtime_error;
 }
@@ -461,6 +463,8 @@ dnnl_status_t dnnl_b200_kv_cache_attention_primitive_desc_create(dnnl_primitive_
     if (query_desc->dims[0] != dst_desc->dims[0] || query_desc->dims[1] != dst_desc->dims[1]) return dnnl_invalid_arguments;
     if (query_desc->dims[1] < 1 || query_desc->dims[1] % cache_desc->dims[1] != 0) return dnnl_invalid_arguments;
     if (cache_desc->dims[3] > 256 || query_desc->dims[1] > 65535) return dnnl_unimplemented;
+    // query rows of a key head are counted in 32 bits
+    if (query_desc->dims[0] * (query_desc->dims[1] / cache_desc->dims[1]) > 0x7fffff00) return dnnl_unimplemented;
     pd_ptr pd = new_pd(dnnl_b200_kv_cache_attention, engine, attr);
     pd->src = *query_desc;
     pd->dst = *dst_desc;

@@ -22,6 +22,11 @@
 
 #include <type_traits>
 
+//
+// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 122 us, e4m3 114 us (574 MB: 4.7
+// and 5.0 TB/s); one of 131009 tokens: 65 us (4.1 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
+// cycle and scheduler: three blocks of four warps per SM are what registers and rings allow (two blocks: 150 us), and
+// the loops wait for their own results more than for memory.
 namespace b200 {
 namespace kv_mma {
 
@@ -121,7 +126,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     const b200_kv_cache_t &c = p.cache;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     part_t line;
-    if (!begin_part<ROWS, EXTRA>(p, line, line_words)) return;
+    if (!begin_part<ROWS, EXTRA, 1>(p, line, line_words)) return;
     const int heads = line.heads, group = line.group, page = (int)c.page, pieces = (int)c.dim / 16;
     uint8_t *ring = smem + warp * S::RING;
     uint2 *q_shared = (uint2 *)(smem + WARPS * S::RING);

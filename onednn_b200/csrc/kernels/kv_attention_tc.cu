@@ -24,6 +24,12 @@
 // most rescaling of O) and to `ref`, a power of two above all value scales.  FINE (f16 results): what P's rounding left
 // is multiplied too.
 //
+// Measured on one B200: three sequences with 1450, 1029 and 1710 new tokens on 5750, 4647 and 3543, 32 query heads on 8, dim 128, s8,
+// bf16: 338 us, 782 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
+// alone take 1.3.  What is left: a softmax step of 64 columns takes a warp 2000 cycles, two of the three warps on a
+// scheduler; items begin and end (8 us each) and cut ones are joined (10 us).  Not kept: 16 softmax warps, two threads per row
+// (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
+//
 // Every wait is bounded; one that runs out sets a bit in the stream's status word and all roles leave.
 #include "kv_line.cuh"
 #include "launch.hpp"
@@ -39,6 +45,7 @@ constexpr int SOFTMAX_WARPS = 8, CONVERT_WARPS = 4, MMA_WARP = SOFTMAX_WARPS + C
 constexpr int REGS = 128, SOFTMAX_REGS = 176, CONVERT_REGS = 104, MMA_REGS = 56;
 static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * REGS && THREADS * REGS <= 65536, "");
 constexpr int EXTRA = 3;   // units that an item's queries, filling and draining, and result take besides (8 of 2.5 us)
+constexpr int MIN_PART = 2; // units; 2 sequences x 8 tokens over 2600 took 46, 41, 39, 41 us with 1, 2, 4, 6, three short prompts 33, 33, 35, 45
 constexpr int STAGES = 2;  // of keys and of values
 constexpr int CHUNKS = UNIT / 16;
 constexpr int STEP = 64, STEPS = UNIT / STEP; // tokens of a step; steps of a unit, which the converters work on
@@ -271,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     uint32_t *status = c.status;
 
     part_t line;
-    if (!begin_part<ROWS, EXTRA>(p, line, ctrl->line_words)) return;
+    if (!begin_part<ROWS, EXTRA, MIN_PART>(p, line, ctrl->line_words)) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctrl->q_full[i], SOFTMAX_WARPS / 2);
@@ -885,10 +892,12 @@ extern "C" B200_API size_t b200_kv_attention_tc_scratch_bytes(const b200_kv_atte
 }
 
 extern "C" B200_API int b200_kv_attention_tc_supported(const b200_kv_attention_params_t *p) {
-    // what the other kernel takes, with pages of whole runs of 16 tokens, and more query rows per sequence and key head
-    // than its items hold
+    // what the other kernel takes, with pages of whole runs of 16 tokens
     if (!b200_kv_attention_mma_supported(p) || p->cache.dim > 128 || p->cache.page % 16) return 0;
-    return p->cache.seqs > 0 && p->cache.heads > 0 && p->rows / p->cache.seqs * (p->q_heads / p->cache.heads) > 32;
+    // and at least 48 query rows per sequence and key head: a tile costs the same however many of its rows there are.  16
+    // sequences of 700 to 4500 tokens, 8 query heads on each of 5 key heads: 32 rows take 50 us there and 61 here, 48 rows 61 and
+    // 62, 64 rows 74 and 62, 128 rows 130 and 62.
+    return p->cache.seqs > 0 && p->cache.heads > 0 && p->rows / p->cache.seqs * (p->q_heads / p->cache.heads) >= 48;
 }
 
 extern "C" B200_API int b200_kv_attention_tc_launch(const b200_kv_attention_params_t *p, b200_stream_t stream) {

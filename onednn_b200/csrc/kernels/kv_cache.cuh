@@ -41,6 +41,7 @@ inline bool kv_cache_ok(const b200_kv_cache_t &c) {
     if (c.dt != B200_DT_S8 && c.dt != B200_DT_F8_E4M3) return false;
     if (c.pages < 0 || c.pages > 0x7fffffff || c.heads < 1 || c.heads > 65535 || c.page < 1 || c.page > (1 << 20) || c.dim < 1)
         return false;
+    if (c.dim > (1 << 20) || c.page * c.dim > (1 << 30) || c.heads * c.dim > (1 << 30)) return false; // counted in 32 bits
     if (c.seqs < 0 || c.seqs > (1 << 24) || c.table_cols < 0) return false;
     if (c.seqs > 0 && (!c.offsets || !c.lens || (c.table_cols > 0 && !c.table))) return false;
     return c.pages == 0 || (c.key && c.value && c.key_scale && c.value_scale);

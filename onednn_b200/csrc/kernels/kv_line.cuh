@@ -104,7 +104,7 @@ struct place_t {
 };
 
 // All threads of the block.  False: the block has no part.  `shared`: LINE_WORDS words that nothing else uses meanwhile.
-template <int ROWS, int EXTRA>
+template <int ROWS, int EXTRA, int MIN_PART>
 __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, part_t &l, int64_t *shared) {
     const b200_kv_cache_t &c = p.cache;
     const int tid = threadIdx.x, threads = blockDim.x;
@@ -127,9 +127,8 @@ __device__ __forceinline__ bool begin_part(const b200_kv_attention_params_t &p, 
     };
     l.total = 0;
     for (int base = 0; base < c.seqs; base += threads) l.total += scan(base);
-    // As many parts as units, if there are blocks for them: parts of at least two or four units were slower (four short
-    // sequences 14 and 16 us instead of 12), the joining costs less than a second unit.
-    l.blocks = (int)min((int64_t)gridDim.x, l.total);
+    // a part has MIN_PART units at least: what it takes to join it is to be less than what it saves
+    l.blocks = (int)min((int64_t)gridDim.x, (l.total + MIN_PART - 1) / MIN_PART);
     if (blockIdx.x >= l.blocks) return false;
     l.begin = l.total * blockIdx.x / l.blocks;
     l.stop = l.total * (blockIdx.x + 1) / l.blocks;

@@ -112,6 +112,10 @@ def test_cache_descriptors_and_refusals(eng):
     refused("invalid_arguments", attend, eng, q, c, md((6, 4, 64), "bf16"), t, 1.0)
     refused("invalid_arguments", attend, eng, q, c, q, t, math.inf)
     refused("unimplemented", attend, eng, md((6, 2, 272), "bf16"), md((5, 2, 16, 272), "s8"), md((6, 2, 272), "bf16"), t, 1.0)
+    # sizes that 32-bit counts inside the kernels do not hold
+    for pages, h, page, dim in ((1, 1, 1 << 20, 2048), (1, 65535, 1, 1 << 15), (1, 1, (1 << 20) + 1, 16), (1, 65536, 1, 16)):
+        refused("unimplemented", read, eng, md((pages, h, page, dim), "s8"), md((1, h, dim), "bf16"), t)
+    refused("unimplemented", attend, eng, md((1 << 30, 4, 64), "bf16"), md((5, 2, 16, 64), "s8"), md((1 << 30, 4, 64), "bf16"), t, 1.0)
     a = api.PrimitiveAttr()
     po = api.PostOps()
     po.append_eltwise(0x20)

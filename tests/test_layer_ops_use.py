@@ -27,8 +27,8 @@ def _impls(eng, rows, seqs, heads=2, group=4, page=16, dim=64, q="bf16", dst=Non
 def test_attention_dispatch(eng):
     """Prompts on tcgen05, steps on mma.sync, whatever neither takes on the generic kernel, which every list ends with."""
     assert _impls(eng, 8, 8) == [MMA, GENERIC]
-    assert _impls(eng, 72, 8, group=4) == [TC, MMA, GENERIC]        # 9 tokens x 4 heads: more than 32 rows
-    assert _impls(eng, 64, 8, group=4) == [MMA, GENERIC]            # 32 rows
+    assert _impls(eng, 96, 8, group=4) == [TC, MMA, GENERIC]        # 12 tokens x 4 heads: 48 rows
+    assert _impls(eng, 95, 8, group=4) == [MMA, GENERIC]
     assert _impls(eng, 100, 1, page=24) == [MMA, GENERIC]           # pages that 16 does not divide
     assert _impls(eng, 100, 1, dim=144) == [MMA, GENERIC]           # heads wider than 128
     assert _impls(eng, 100, 1, dim=256, cache="e4m3") == [MMA, GENERIC]
