@@ -294,10 +294,16 @@ dnnl_status_t attention_execute(const dnnl_primitive *prim, dnnl_stream *stream,
         return status_of(impl->launch(&p, cs));
     }
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(cs, &capture) != cudaSuccess) return dnnl_runtime_error;
+    if (cudaStreamIsCapturing(cs, &capture) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return dnnl_runtime_error;
+    }
     if (capture != cudaStreamCaptureStatusNone) {
         // a graph may be replayed next to others and to eager executions: it gets memory of its own
-        if (device_alloc_async(&p.scratch, p.scratch_bytes, cs) != cudaSuccess) return dnnl_out_of_memory;
+        if (device_alloc_async(&p.scratch, p.scratch_bytes, cs) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return dnnl_out_of_memory;
+        }
         const dnnl_status_t st = status_of(impl->launch(&p, cs));
         if (cudaFreeAsync(p.scratch, cs) != cudaSuccess) return dnnl_runtime_error;
         return st;
