@@ -367,7 +367,7 @@ B200_API int b200_kv_attention_mma_supported(const b200_kv_attention_params_t *p
 B200_API size_t b200_kv_attention_mma_scratch_bytes(const b200_kv_attention_params_t *p);
 B200_API int b200_kv_attention_mma_launch(const b200_kv_attention_params_t *p, b200_stream_t stream);
 
-/* Many query rows per key head, on tcgen05: as above, with dim up to 128, pages of a multiple of 16 tokens, and at
+/* Many query rows per key head, on tcgen05: as above, with dim up to 128, pages of a multiple of 8 tokens, and at
  * least 48 query rows per sequence and key head on average. */
 B200_API int b200_kv_attention_tc_supported(const b200_kv_attention_params_t *p);
 B200_API size_t b200_kv_attention_tc_scratch_bytes(const b200_kv_attention_params_t *p);

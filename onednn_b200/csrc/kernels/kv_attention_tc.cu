@@ -17,10 +17,10 @@
 //                    look at a barrier some 300.)
 //   warp 14          finds the block's items ahead of all others and lays them out in shared memory
 //
-// The two scales stay out of the products.  A page holds a multiple of 16 tokens here, so 16 neighbouring tokens share
-// theirs: x = s * (key scale * softmax scale), and the value scale enters the exponent,
+// The two scales stay out of the products.  A page holds a multiple of RUN (16 or 8) tokens here, so as many neighbouring tokens
+// share theirs: x = s * (key scale * softmax scale), and the value scale enters the exponent,
 // P = 2^(x - m + log2(value scale) - ref), so neither costs an operation per element; the sum takes P back by a
-// factor per 16 tokens.  P is f16 relative to 2^8 (m follows the maximum only when that has grown by more, which saves
+// factor per run.  P is f16 relative to 2^8 (m follows the maximum only when that has grown by more, which saves
 // most rescaling of O) and to `ref`, a power of two above all value scales.  FINE (f16 results): what P's rounding left
 // is multiplied too.
 //
@@ -47,7 +47,6 @@ static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + MMA_REGS <= 4 * REGS && THREADS 
 constexpr int EXTRA = 3;   // units that an item's queries, filling and draining, and result take besides (8 of 2.5 us)
 constexpr int MIN_PART = 2; // units; 2 sequences x 8 tokens over 2600 took 46, 41, 39, 41 us with 1, 2, 4, 6, three short prompts 33, 33, 35, 45
 constexpr int STAGES = 2;  // of keys and of values
-constexpr int CHUNKS = UNIT / 16;
 constexpr int STEP = 64, STEPS = UNIT / STEP; // tokens of a step; steps of a unit, which the converters work on
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t WAIT_TRIES = 1u << 19; // of up to 2 us each, suspended in hardware
@@ -59,11 +58,11 @@ struct smem_t {
     static constexpr int BYTES = (2 + 2 * STAGES) * MAT;
 };
 
-// The scales of a tile's tokens, 16 at a time, as the softmax takes them.  Four tiles deep: the converters are at most
+// The scales of a tile's tokens, run by run, as the softmax takes them.  Four tiles deep: the converters are at most
 // two ahead of the slower softmax.
 struct scales_t {
     // x key scale, y 0 (-inf: no such page), z log2(value scale) - ref (-inf: no such page), w 2^-z
-    float4 chunk[CHUNKS];
+    float4 chunk[UNIT / 8];
     float step; // what O is to be multiplied by: 2^(last tile's ref - this one's)
     float up;   // 2^ref
 };
@@ -265,9 +264,10 @@ __device__ __forceinline__ uint32_t piece_at(int row, int piece) {
     return (uint32_t)((piece >> 3) * (UNIT * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
-template <int DP, bool S8, bool FINE>
+template <int DP, bool S8, bool FINE, int RUN>
 __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
     using S = smem_t<DP>;
+    constexpr int CHUNKS = UNIT / RUN; // runs of a unit
     extern __shared__ uint8_t smem_raw[];
     __shared__ ctrl_t ctrl_mem;
     ctrl_t *ctrl = &ctrl_mem;
@@ -434,13 +434,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     tc_fence_after();
                     if (j + 1 == steps) fetch_next();
                     const scales_t &sc = ctrl->scales[(tile_i + j / STEPS) & 3];
-                    const float4 *chunk = sc.chunk + place * (STEP / 16);
+                    const float4 *chunk = sc.chunk + place * (STEP / RUN);
                     const uint32_t tmem_p = tmem_s + place * STEP;
                     // ---- the scores, and the largest
                     uint32_t v[2][32];
-                    float4 ck[4];
+                    float4 ck[STEP / RUN];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) ck[k] = chunk[k];
+                    for (int k = 0; k < STEP / RUN; ++k) ck[k] = chunk[k];
                     const float step = place == 0 ? sc.step : 1.f;
                     up = sc.up;
                     tmem_ld32_issue(tmem_p, v[0]);
@@ -453,20 +453,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         for (int i = 0; i < STEP; ++i)
                             if (i > seen) v[i >> 5][i & 31] = 0xff800000u;
                     }
-                    float f[4], top = m;
+                    float f[STEP / RUN], top = m;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t *y = v[k >> 1] + (k & 1) * 16;
+                    for (int k = 0; k < STEP / RUN; ++k) {
+                        const uint32_t *y = v[k * RUN >> 5] + (k * RUN & 31);
                         float x0 = max3(__uint_as_float(y[0]), __uint_as_float(y[1]), __uint_as_float(y[2]));
-                        float x1 = max3(__uint_as_float(y[8]), __uint_as_float(y[9]), __uint_as_float(y[10]));
+                        float x1 = max3(__uint_as_float(y[RUN / 2]), __uint_as_float(y[RUN / 2 + 1]), __uint_as_float(y[RUN / 2 + 2]));
 #pragma unroll
-                        for (int i = 3; i < 7; i += 2) {
+                        for (int i = 3; i + 1 < RUN / 2; i += 2) {
                             x0 = max3(x0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
-                            x1 = max3(x1, __uint_as_float(y[8 + i]), __uint_as_float(y[9 + i]));
+                            x1 = max3(x1, __uint_as_float(y[RUN / 2 + i]), __uint_as_float(y[RUN / 2 + i + 1]));
                         }
-                        x0 = max3(x0, x1, __uint_as_float(y[7]));
+                        x0 = max3(x0, x1, __uint_as_float(y[RUN / 2 - 1]));
                         f[k] = ck[k].x * factor;
-                        top = fmaxf(top, fmaf(fmaxf(x0, __uint_as_float(y[15])), f[k], ck[k].y));
+                        top = fmaxf(top, fmaf(fmaxf(x0, __uint_as_float(y[RUN - 1])), f[k], ck[k].y));
                     }
                     // ---- m and ref follow, seldom; O and the sum with them
                     const bool follow = top > m + 8.f; // also from -inf
@@ -490,28 +490,32 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     // ---- weights, over the scores: of each 16 columns the first eight, FINE: the other eight too
                     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t *y = v[k >> 1] + (k & 1) * 16;
-                        const float off = ck[k].z - base;
-                        const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(off, off);
-                        uint64_t sum = 0;
+                    for (int h = 0; h < STEP / 16; ++h) {
                         uint32_t pw[FINE ? 16 : 8];
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const float2 x = unpack2(fma2(f32x2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), ff, oo));
-                            const float e0 = ex2(x.x), e1 = ex2(x.y);
-                            sum = add2(sum, f32x2(e0, e1));
-                            const uint32_t hi = pack_f16x2(e0, e1);
-                            pw[i / 2] = hi;
-                            if (FINE) {
-                                const float2 had = f16x2_to_f32(hi);
-                                pw[FINE ? 8 + i / 2 : 0] = pack_f16x2(e0 - had.x, e1 - had.y);
+                        for (int k = h * 16 / RUN; k < (h + 1) * 16 / RUN; ++k) {
+                            const uint32_t *y = v[k * RUN >> 5] + (k * RUN & 31);
+                            const float off = ck[k].z - base;
+                            const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(off, off);
+                            uint64_t sum = 0;
+#pragma unroll
+                            for (int i = 0; i < RUN; i += 2) {
+                                const int at = (k * RUN % 16 + i) / 2;
+                                const float2 x = unpack2(fma2(f32x2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), ff, oo));
+                                const float e0 = ex2(x.x), e1 = ex2(x.y);
+                                sum = add2(sum, f32x2(e0, e1));
+                                const uint32_t hi = pack_f16x2(e0, e1);
+                                pw[at] = hi;
+                                if (FINE) {
+                                    const float2 had = f16x2_to_f32(hi);
+                                    pw[FINE ? 8 + at : 0] = pack_f16x2(e0 - had.x, e1 - had.y);
+                                }
                             }
+                            const float2 both = unpack2(sum);
+                            l = fmaf(both.x + both.y, ck[k].w, l);
                         }
-                        const float2 both = unpack2(sum);
-                        l = fmaf(both.x + both.y, ck[k].w, l);
-                        if (FINE) tmem_st16(tmem_p + k * 16, pw);
-                        else tmem_st8(tmem_p + k * 16, pw);
+                        if (FINE) tmem_st16(tmem_p + h * 16, pw);
+                        else tmem_st8(tmem_p + h * 16, pw);
                     }
                     tmem_wait_st();
                     tc_fence_before();
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     } else if (warp < MMA_WARP) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CONVERT_REGS));
         // ---------------- codes to f16 ----------------
-        // Warp w has tokens 32 w .. of a tile: two runs of 16, each in one page.  An access of the warp covers 512 / DP tokens in
+        // Warp w has tokens 32 w .. of a tile: runs of RUN, each in one page.  An access of the warp covers 512 / DP tokens in
         // groups of eight lanes: two tokens, 64 dims each, so that both the 64-byte reads and the stores (pieces
         // 0, 2, 4, 6 of an even token, swizzled, and of the odd one next to it) use all that they touch.
         constexpr int CH = DP / 16, PER = 32 / CH, LOADS = 32 / PER;
@@ -644,14 +648,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             give_back(seg_i++);
             const uint8_t *keys = (const uint8_t *)c.key + head * c.s_head + cc * 16, *values = (const uint8_t *)c.value + head * c.s_head + cc * 16;
             uint4 kr[LOADS], vr[LOADS];
-            // every warp looks up all eight runs of a tile, one per lane, because `ref` needs all their scales
+            // every warp looks up all runs of a tile, one per lane, because `ref` needs all their scales
             int64_t place = -1;
             float ks = -1.f, vs = 0.f;
-            int n = (u0 * UNIT + lane * 16) / page, slot = u0 * UNIT + lane * 16 - n * page;
+            int n = (u0 * UNIT + lane * RUN) / page, slot = u0 * UNIT + lane * RUN - n * page;
             const int jump_n = UNIT / page, jump_slot = UNIT - jump_n * page;
             auto find = [&](int j) {
                 place = -1, ks = -1.f, vs = 0.f;
-                if (lane < CHUNKS && j < u1 && j * UNIT + lane * 16 < end) {
+                if (lane < CHUNKS && j < u1 && j * UNIT + lane * RUN < end) {
                     const int phys = table[n];
                     if (phys >= 0 && phys < c.pages) {
                         place = (int64_t)phys * c.s_page + (int64_t)slot * c.s_slot;
@@ -665,21 +669,26 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 if (slot >= page) slot -= page, ++n;
             };
             auto load = [&](int j, const uint8_t *from, uint4 (&regs)[LOADS]) {
-                const int64_t run[2] = {__shfl_sync(~0u, place, w * 2), __shfl_sync(~0u, place, w * 2 + 1)};
+                int64_t run[32 / RUN], worst = 0;
+#pragma unroll
+                for (int k = 0; k < 32 / RUN; ++k) {
+                    run[k] = __shfl_sync(~0u, place, w * (32 / RUN) + k);
+                    worst |= run[k];
+                }
                 const int left = end - j * UNIT - w * 32;
-                if (DP == c.dim && (run[0] | run[1]) >= 0 && left >= 32) { // all there
-                    const uint8_t *at_run[2] = {from + run[0] + lane_at, from + run[1] + lane_at};
+                static_assert(RUN % PER == 0, "an access stays in its run");
+                if (DP == c.dim && worst >= 0 && left >= 32) { // all there
 #pragma unroll
                     for (int i = 0; i < LOADS; ++i) // a run's accesses are PER tokens apart
-                        regs[i] = __ldg((const uint4 *)(at_run[i * PER >> 4] + (i % (16 / PER)) * per_step));
+                        regs[i] = __ldg((const uint4 *)(from + run[i * PER / RUN] + lane_at + (i % (RUN / PER)) * per_step));
                     return;
                 }
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
                     const int tok = i * PER + sub_row; // of the warp's 32; the run is known at compile time
                     regs[i] = make_uint4(0, 0, 0, 0);
-                    if (takes && run[i * PER >> 4] >= 0 && tok < left)
-                        regs[i] = __ldg((const uint4 *)(from + run[i * PER >> 4] + (tok & 15) * c.s_slot));
+                    if (takes && run[i * PER / RUN] >= 0 && tok < left)
+                        regs[i] = __ldg((const uint4 *)(from + run[i * PER / RUN] + (tok & (RUN - 1)) * c.s_slot));
                 }
             };
             auto convert = [&](const uint4 (&regs)[LOADS], uint8_t *to) {
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 const float log = lg2(fmaxf(vs, 7.5231638e-37f)); // 2^-120 at least
                 float top = lane < CHUNKS ? log : -200.f;
 #pragma unroll
-                for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+                for (int o = CHUNKS / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
                 top = __shfl_sync(~0u, top, 0);
                 // with room, so that it seldom moves
                 const float now = top > ref ? ceilf(top) + 1.f : ref;
@@ -865,14 +874,18 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
     }
 }
 
-template <int DP, bool S8, bool FINE>
+template <int DP, bool S8, bool FINE, int RUN>
 int run(const b200_kv_attention_params_t &p, cudaStream_t cs) {
-    auto kernel = kv_attention_tc_kernel<DP, S8, FINE>;
+    auto kernel = kv_attention_tc_kernel<DP, S8, FINE, RUN>;
     const int bytes = smem_t<DP>::BYTES + 1024;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return (int)e;
     kernel<<<p.sm_count, THREADS, bytes, cs>>>(p);
     return after_launch();
+}
+template <int DP, bool S8, bool FINE>
+int run(const b200_kv_attention_params_t &p, cudaStream_t cs) {
+    return p.cache.page % 16 == 0 ? run<DP, S8, FINE, 16>(p, cs) : run<DP, S8, FINE, 8>(p, cs);
 }
 template <int DP, bool S8>
 int run(const b200_kv_attention_params_t &p, cudaStream_t cs) {
@@ -892,8 +905,8 @@ extern "C" B200_API size_t b200_kv_attention_tc_scratch_bytes(const b200_kv_atte
 }
 
 extern "C" B200_API int b200_kv_attention_tc_supported(const b200_kv_attention_params_t *p) {
-    // what the other kernel takes, with pages of whole runs of 16 tokens
-    if (!b200_kv_attention_mma_supported(p) || p->cache.dim > 128 || p->cache.page % 16) return 0;
+    // what the other kernel takes, with pages of whole runs of 8 tokens
+    if (!b200_kv_attention_mma_supported(p) || p->cache.dim > 128 || p->cache.page % 8) return 0;
     // and at least 48 query rows per sequence and key head: a tile costs the same however many of its rows there are.  16
     // sequences of 700 to 4500 tokens, 8 query heads on each of 5 key heads: 32 rows take 50 us there and 61 here, 48 rows 61 and
     // 62, 64 rows 74 and 62, 128 rows 130 and 62.

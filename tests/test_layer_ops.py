@@ -617,6 +617,9 @@ ATTEND = [  # lens, news, heads, group, page, dim, cache kind, q kind, before, b
     ([900, 10, 0], [257, 20, 3], 1, 4, 128, 128, "e4m3", "f16", 2, 0),  # rows that see no token
     ([5000], [64], 2, 1, 32, 128, "s8", "bf16", 0, 0),  # one item in many parts
     ([2100, 2100], [700, 650], 3, 2, 16, 80, "s8", "bf16", 0, 0),
+    ([300, 77, 129], [150, 77, 129], 2, 2, 8, 128, "s8", "bf16", 0, 0),  # runs of 8 tokens
+    ([1000, 300], [200, 300], 1, 4, 24, 64, "e4m3", "f16", 1, 1),
+    ([613], [333], 2, 1, 200, 112, "e4m3", "bf16", 0, 0),
     ([50] * 70, [1] * 70, 1, 8, 16, 64, "s8", "bf16", 0, 0),
 ]
 

@@ -29,7 +29,8 @@ def test_attention_dispatch(eng):
     assert _impls(eng, 8, 8) == [MMA, GENERIC]
     assert _impls(eng, 96, 8, group=4) == [TC, MMA, GENERIC]        # 12 tokens x 4 heads: 48 rows
     assert _impls(eng, 95, 8, group=4) == [MMA, GENERIC]
-    assert _impls(eng, 100, 1, page=24) == [MMA, GENERIC]           # pages that 16 does not divide
+    assert _impls(eng, 100, 1, page=24) == [TC, MMA, GENERIC]
+    assert _impls(eng, 100, 1, page=20) == [MMA, GENERIC]           # pages that 8 does not divide
     assert _impls(eng, 100, 1, dim=144) == [MMA, GENERIC]           # heads wider than 128
     assert _impls(eng, 100, 1, dim=256, cache="e4m3") == [MMA, GENERIC]
     assert _impls(eng, 100, 1, dim=72) == [GENERIC]                 # rows of codes that 16 bytes do not divide
