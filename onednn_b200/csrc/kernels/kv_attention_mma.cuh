@@ -61,6 +61,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)_
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -176,6 +179,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         };
         int64_t place = -1; // of the lane's tokens in the step that is being copied
         int place_page = 0;
+        bool simple = false; // all tokens are there, and rows lie densely: addresses are constants apart
         auto find = [&](int step) {
             place = -1;
             place_page = next_page;
@@ -183,6 +187,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                 if (next_page >= 0 && next_page < c.pages) place = (int64_t)next_page * c.s_page + (int64_t)next_slot * c.s_slot;
                 else flag_bad_page(c);
             }
+            if (RUNS) simple = __all_sync(~0u, place >= 0) && (step + 1) * STEP <= end && c.s_slot == DP && c.dim == DP;
         };
         // keys (VAL false) or values of a step into a half stage, their scales behind them
         auto copy = [&](auto val, int step, uint8_t *to) {
@@ -190,6 +195,14 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             const uint8_t *from = VAL ? values : keys;
             float *scales = (float *)(to + STEP * DP);
             const int left = end - step * STEP; // tokens of this step and behind
+            if (RUNS && simple) {
+                cp4(smem_u32(scales + lane), (VAL ? c.value_scale : c.key_scale) + (int64_t)place_page * heads + head);
+                const uint8_t *f = from + place + lane % CH * 16;
+                const uint32_t d = smem_u32(to + lead * DP);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) cp16(d + i * DP + (VAL ? value_piece<DP>(i, lane % CH) : key_piece<DP>(i, lane % CH)) * 16, f + i * DP);
+                return;
+            }
             if (place >= 0 && lane < left) cp4(smem_u32(scales + lane), (VAL ? c.value_scale : c.key_scale) + (int64_t)place_page * heads + head);
             else scales[lane] = VAL ? 0.f : -1.f; // no such token
             const int cc = lane % CH;

@@ -621,6 +621,9 @@ ATTEND = [  # lens, news, heads, group, page, dim, cache kind, q kind, before, b
     ([1000, 300], [200, 300], 1, 4, 24, 64, "e4m3", "f16", 1, 1),
     ([613], [333], 2, 1, 200, 112, "e4m3", "bf16", 0, 0),
     ([50] * 70, [1] * 70, 1, 8, 16, 64, "s8", "bf16", 0, 0),
+    ([1 + i * 37 % 200 for i in range(300)], [i % 3 for i in range(300)], 2, 2, 16, 64, "s8", "bf16", 0, 0),  # more than a block's threads
+    ([30 + i * 7 % 90 for i in range(530)], [30 if i % 5 else 0 for i in range(530)], 1, 2, 16, 64, "s8", "f16", 1, 0),
+    ([3000] + [2] * 130, [700] + [1] * 130, 1, 2, 8, 128, "e4m3", "bf16", 0, 0),  # a prompt among steps
 ]
 
 
