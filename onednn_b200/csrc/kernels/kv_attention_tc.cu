@@ -49,7 +49,8 @@ constexpr int MIN_PART = 2; // units; 2 sequences x 8 tokens over 2600 took 46, 
 constexpr int STAGES = 2;  // of keys and of values
 constexpr int STEP = 64, STEPS = UNIT / STEP; // tokens of a step; steps of a unit, which the converters work on
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t WAIT_TRIES = 1u << 19; // of up to 2 us each, suspended in hardware
+constexpr uint32_t WAIT_TRIES = 1u << 30;
+constexpr uint64_t WAIT_NS = 4000000000ull; // a warp without rows waits through the other tile's whole segment, which takes milliseconds at most
 enum : uint32_t { ST_WAIT = 0x00100000 };
 
 template <int DP>
@@ -112,14 +113,23 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity) {
             : "memory");
     return ok != 0;
 }
-// false when the wait ran out or another role gave up; the same for all lanes that wait together
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// false when the wait ran out (by the clock) or another role gave up; the same for all lanes that wait together
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, ctrl_t *c, uint32_t *status) {
+    if (mbar_try(bar, parity)) return true;
+    const uint64_t until = now_ns() + WAIT_NS;
     for (uint32_t i = 0; i < WAIT_TRIES; ++i) {
         if (mbar_try(bar, parity)) return true;
-        if (c->abort) return false;
+        if (c->abort || ((i & 255) == 255 && now_ns() > until)) break;
     }
-    c->abort = 1;
-    if (status) atomicOr(status, (uint32_t)ST_WAIT);
+    if (!c->abort) {
+        c->abort = 1;
+        if (status) atomicOr(status, (uint32_t)ST_WAIT);
+    }
     return false;
 }
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, ctrl_t *c, uint32_t *status) {
