@@ -23,8 +23,8 @@
 #include <type_traits>
 
 //
-// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 122 us, e4m3 114 us (574 MB: 4.7
-// and 5.0 TB/s); one of 131009 tokens: 65 us (4.1 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
+// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 117 us, e4m3 113 us (574 MB: 4.9
+// and 5.1 TB/s); one of 131009 tokens: 64 us (4.2 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
 // cycle and scheduler: three blocks of four warps per SM are what registers and rings allow (two blocks: 150 us), and
 // the loops wait for their own results more than for memory.
 namespace b200 {

@@ -25,7 +25,7 @@
 // is multiplied too.
 //
 // Measured on one B200: three sequences with 1450, 1029 and 1710 new tokens on 5750, 4647 and 3543, 32 query heads on 8, dim 128, s8,
-// bf16: 338 us, 782 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
+// bf16: 328 us, 806 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
 // alone take 1.3.  What is left: a softmax step of 64 columns takes a warp 2000 cycles, two of the three warps on a
 // scheduler; items begin and end (8 us each) and cut ones are joined (10 us).  Not kept: 16 softmax warps, two threads per row
 // (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
@@ -49,7 +49,7 @@ constexpr int MIN_PART = 2; // units; 2 sequences x 8 tokens over 2600 took 46, 
 constexpr int STAGES = 2;  // of keys and of values
 constexpr int STEP = 64, STEPS = UNIT / STEP; // tokens of a step; steps of a unit, which the converters work on
 constexpr uint32_t TMEM_COLS = 512;
-constexpr uint32_t WAIT_TRIES = 1u << 30;
+constexpr uint32_t WAIT_TRIES = 1u << 30; // the clock ends a wait long before
 constexpr uint64_t WAIT_NS = 4000000000ull; // a warp without rows waits through the other tile's whole segment, which takes milliseconds at most
 enum : uint32_t { ST_WAIT = 0x00100000 };
 
