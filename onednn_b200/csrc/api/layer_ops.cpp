@@ -291,6 +291,7 @@ dnnl_status_t attention_execute(const dnnl_primitive *prim, dnnl_stream *stream,
         auto it = args.find(DNNL_ARG_SCRATCHPAD);
         if (it == args.end() || !it->second->handle || it->second->md.size_bytes() < p.scratch_bytes) return dnnl_invalid_arguments;
         p.scratch = at(args, DNNL_ARG_SCRATCHPAD);
+        if ((uintptr_t)p.scratch % 16 != 0) return dnnl_invalid_arguments; // partial results are read 16 bytes at a time
         return status_of(impl->launch(&p, cs));
     }
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
@@ -345,7 +346,15 @@ dnnl_status_t ext_execute(const dnnl_primitive *prim, dnnl_stream *stream, const
         auto it = args.find(want.first);
         if (it == args.end() || !it->second->md.equal(want.second)) return dnnl_invalid_arguments;
         if (!it->second->handle && !want.second.has_zero_dim()) return dnnl_invalid_arguments;
+        // no element may straddle its type's boundary: a kernel that read it would fault
+        if ((uintptr_t)it->second->handle % (dt_nbits(want.second.data_type) / 8) != 0) return dnnl_invalid_arguments;
     }
+    // blocks of the append write keys and values side by side: in one place they would race
+    if (pd->kind == dnnl_b200_kv_cache_append
+            && (at(args, DNNL_ARG_B200_KEY_SCALES) == at(args, DNNL_ARG_B200_VALUE_SCALES)
+                    || at(args, DNNL_ARG_B200_KEY_CACHE) == at(args, DNNL_ARG_B200_VALUE_CACHE))
+            && !pd->dst.has_zero_dim())
+        return dnnl_invalid_arguments;
     switch (pd->kind) {
         case dnnl_b200_rms_norm: return norm_execute(pd, stream, args);
         case dnnl_b200_kv_cache_attention: return attention_execute(prim, stream, args);

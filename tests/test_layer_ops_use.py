@@ -391,6 +391,65 @@ def test_buffers_that_vector_accesses_cannot_start_at(gpu, spec):
 
 
 @pytest.mark.gpu
+def test_addresses_within_an_element_are_refused(gpu):
+    """Refused on the host: a buffer that starts inside an element of its type, a scratchpad that 16 bytes do not divide."""
+    torch, _ = T._torch()
+    e, s = gpu
+    c, q = _case(STEP)
+    dst = torch.zeros_like(q)
+    a = api.PrimitiveAttr()
+    a.set_scratchpad_mode(1)
+    pd = api.kv_cache_attention_primitive_desc(e, tmd(q), tmd(c.codes[0]), tmd(dst), tmd(c.table), 0.1, attr=a)
+    n = pd.scratchpad_desc().get_size()
+    buf = torch.zeros(n + 1024, dtype=torch.uint8, device="cuda")
+    p = api.Primitive(pd)
+    args = {**c.args(e), api.ARG_SRC: mem(q, e), api.ARG_DST: mem(dst, e),
+            api.ARG_SCRATCHPAD: api.Memory(pd.scratchpad_desc(), e, buf.data_ptr())}
+
+    def refused(prim, a):
+        with pytest.raises(api.Error) as err:
+            prim.execute(s, a)
+        assert err.value.name == "invalid_arguments"
+    for off in (1, 4, 8):
+        refused(p, {**args, api.ARG_SCRATCHPAD: api.Memory(pd.scratchpad_desc(), e, buf.data_ptr() + off)})
+    for arg, t in ((api.ARG_SRC, q), (api.ARG_DST, dst), (api.ARG_B200_KEY_SCALES, c.scales[0]), (api.ARG_B200_PAGE_TABLE, c.table),
+                   (api.ARG_B200_SEQ_OFFSETS, c.offsets), (api.ARG_B200_KV_LENS, c.kv_lens)):
+        refused(p, {**args, arg: api.Memory(tmd(t), e, t.data_ptr() + 1)})
+    p.execute(s, args)
+    s.wait()
+    check_attention(c, q, 0.1, dst, dst, "bf16")
+
+    x, y = torch.randn(8, 64, device="cuda"), torch.zeros(8, 64, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(8, device="cuda")
+    norm = api.Primitive(api.rms_norm_primitive_desc(e, tmd(x), tmd(y), 1e-5))
+    where = api.ARG_ATTR_SCALES | api.ARG_DST
+    good = {api.ARG_SRC: mem(x, e), api.ARG_DST: mem(y, e), where: mem(scales, e)}
+    refused(norm, {**good, where: api.Memory(tmd(scales), e, scales.data_ptr() + 2)})
+    refused(norm, {**good, api.ARG_SRC: api.Memory(tmd(x), e, x.data_ptr() + 2)})
+    norm.execute(s, good)
+    s.wait()
+
+
+@pytest.mark.gpu
+def test_append_wants_two_caches(gpu):
+    """Keys and values written into one cache, or two caches with one set of scales, would race."""
+    torch, _ = T._torch()
+    e, s = gpu
+    c = Cache([20, 3], [2, 3], 2, 16, 64, "s8")
+    x = torch.randn(c.rows, 2, 64, generator=c.g, device="cuda")
+    before = [t.clone() for t in c.codes + c.scales]
+    p = api.Primitive(api.kv_cache_append_primitive_desc(e, tmd(x), tmd(c.codes[0]), tmd(c.table)))
+    args = {**c.args(e), api.ARG_SRC: mem(x, e), api.ARG_SRC_1: mem(x, e)}
+    for one, other in ((api.ARG_B200_KEY_CACHE, api.ARG_B200_VALUE_CACHE), (api.ARG_B200_KEY_SCALES, api.ARG_B200_VALUE_SCALES)):
+        with pytest.raises(api.Error) as err:
+            p.execute(s, {**args, other: args[one]})
+        assert err.value.name == "invalid_arguments"
+    s.wait()
+    for was, now in zip(before, c.codes + c.scales):
+        assert torch.equal(T.bits(was), T.bits(now))
+
+
+@pytest.mark.gpu
 def test_a_cache_beyond_four_gigabytes(gpu):
     """Pages whose codes lie behind 2^32 bytes: append, read and both attention kernels find them."""
     torch, _ = T._torch()
