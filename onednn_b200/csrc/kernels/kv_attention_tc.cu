@@ -372,6 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                                  : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
+            __syncwarp(); // loads of tensor memory follow, which a warp issues together
         };
         // The row of an item that `fetch` brought: to f16 after a power of two that brings its largest element to [1, 2).
         // A negative softmax scale turns the query round, so that factors of the scores are positive.
@@ -565,20 +566,22 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 for (int h = 0; h < DP / 32; ++h) {
                     uint32_t v[32];
                     tmem_ld32(tmem_o + h * 32, v);
-                    if (!mine) continue;
+                    if (mine) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        float x[8];
+                        for (int i = 0; i < 32; i += 8) {
+                            float x[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]);
-                        if (whole) {
-                            put(h * 32 + i, x, inv);
-                        } else { // rows side by side, so that a warp's stores are contiguous
-                            float4 *d4 = (float4 *)(part + 2 * ROWS) + (h * 32 + i) / 4 * ROWS + pr;
-                            d4[0] = make_float4(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
-                            d4[ROWS] = make_float4(x[4] * up, x[5] * up, x[6] * up, x[7] * up);
+                            for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]);
+                            if (whole) {
+                                put(h * 32 + i, x, inv);
+                            } else { // rows side by side, so that a warp's stores are contiguous
+                                float4 *d4 = (float4 *)(part + 2 * ROWS) + (h * 32 + i) / 4 * ROWS + pr;
+                                d4[0] = make_float4(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
+                                d4[ROWS] = make_float4(x[4] * up, x[5] * up, x[6] * up, x[7] * up);
+                            }
                         }
                     }
+                    __syncwarp(); // the next load is the whole warp's, lanes without a row among them
                 }
                 tc_fence_before(); // O may be written again after the next arrival
                 if (!whole && mine) part[pr] = m, part[ROWS + pr] = l;
