@@ -88,6 +88,7 @@ struct ctrl_t {
     segment_t segments[SEGMENTS];
     uint64_t q_full[2], s_full[2][STEPS], p_full[2][STEPS], o_done[2][STEPS], join;
     uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
+    uint64_t drained[2];
     uint32_t tmem_base;
     volatile uint32_t abort;
     uint32_t last_part;
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             mbar_init(&ctrl->seg_empty[i], SOFTMAX_WARPS + CONVERT_WARPS + 2);
         }
         mbar_init(&ctrl->join, SOFTMAX_WARPS);
+        for (int i = 0; i < 2; ++i) mbar_init(&ctrl->drained[i], 1);
         ctrl->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -879,8 +881,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             }
         }
     }
-    // all roles are through (the MMAs too: every one was waited for by way of o_done, unless a wait ran out)
+    // All roles are through.  The MMAs too, every one was waited for by way of o_done -- unless a wait ran out: then their
+    // issuers wait for what is still under way, before its operands and results are given up.
     __syncthreads();
+    if (ctrl->abort) {
+        if (warp == MMA_WARP || warp == MMA_WARP + 1) {
+            uint64_t *bar = &ctrl->drained[warp - MMA_WARP];
+            if (elect_one()) tc_commit(bar);
+            __syncwarp();
+            const uint64_t until = now_ns() + WAIT_NS;
+            for (uint32_t i = 0; i < WAIT_TRIES && !mbar_try(bar, 0); ++i)
+                if ((i & 255) == 255 && now_ns() > until) break;
+        }
+        __syncthreads();
+    }
     if (warp == MMA_WARP) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
