@@ -165,17 +165,23 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         const int lead = RUNS ? lane / CH * CH : lane; // the token of a step that this lane looks up
         int next_page = -1, next_j, next_slot;
         const int jump_j = UNIT / page, jump_slot = UNIT - jump_j * page;
+        // steps behind the last one are left out by their number: a token of theirs may not fit 32 bits
+        const int first_step = u0 * WARPS + warp, steps_end = (end + STEP - 1) / STEP;
         auto look_up_at = [&](int step) {
+            next_page = -1, next_j = 0, next_slot = 0;
+            if (step >= steps_end) return;
             const int tok = step * STEP + lead;
             next_j = tok / page;
             next_slot = tok - next_j * page;
-            next_page = tok < end ? table[next_j] : -1;
+            if (tok < end) next_page = table[next_j];
         };
         auto look_up_next = [&](int step) { // the warp's step after the one looked up before
+            next_page = -1;
+            if (step >= steps_end) return;
             next_j += jump_j;
             next_slot += jump_slot;
             if (next_slot >= page) next_slot -= page, ++next_j;
-            next_page = step * STEP + lead < end ? table[next_j] : -1;
+            if (step * STEP + lead < end) next_page = table[next_j];
         };
         int64_t place = -1; // of the lane's tokens in the step that is being copied
         int place_page = 0;
@@ -231,7 +237,6 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         };
         constexpr std::integral_constant<bool, false> KEYS;
         constexpr std::integral_constant<bool, true> VALUES;
-        const int first_step = u0 * WARPS + warp, steps_end = (end + STEP - 1) / STEP;
 #pragma unroll
         for (int i = 0; i < S::STAGES; ++i) {
             const int step = first_step + i * WARPS;
