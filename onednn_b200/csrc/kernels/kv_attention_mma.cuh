@@ -12,9 +12,14 @@
 // f16 exactly (both types fit) in registers; which dim or token an instruction's k index stands for is free as
 // long as both operands agree, so the fragments are chosen to be 16-byte pieces of the rows as they lie in the cache.
 // FINE (f16 results): what a weight's rounding to f16 left is multiplied too; bf16's own last rounding is eight
-// times as large, so there it would not show.  Scales stay out of the products: the key's multiplies the score, the value's the weight.  f16 holds weights
-// relative to the largest to 2^-11: p in [0, 1], times the value scale relative to the largest power of two seen
-// (`ref`); queries are taken to f16 after a power of two per row that brings the largest element to [1, 2).
+// times as large, so there it would not show.
+// Scales stay out of the products: the key's multiplies the score, the value's the weight.  f16 holds weight times
+// value scale, P = 2^(x - m - k + 14) * scale, with two numbers of each row: m, the largest score x that it has seen, and k, a
+// whole number such that no token that it sees has x + log2(scale) above m + k.  So P < 2^14, rounded to 2^-11 of
+// itself down to 2^-28 of that, and no page that a row does not see, or gives no weight, takes bits from the others.  In a
+// step whose scales lie within 2^4 of one another the largest stands for all; else k comes from the tokens one by one.
+// Sum and weighted values are both relative to 2^(m + k - 14).  Queries are taken to f16 after a power of two per row that
+// brings the largest element to [1, 2).
 #pragma once
 
 #include "kv_line.cuh"
@@ -23,8 +28,8 @@
 #include <type_traits>
 
 //
-// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 117 us, e4m3 113 us (574 MB: 4.9
-// and 5.1 TB/s); one of 131009 tokens: 64 us (4.2 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
+// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 120 us, e4m3 116 us (574 MB: 4.8
+// and 4.9 TB/s); one of 131009 tokens: 65 us (4.1 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
 // cycle and scheduler: three blocks of four warps per SM are what registers and rings allow (two blocks: 150 us), and
 // the loops wait for their own results more than for memory.
 namespace b200 {
@@ -34,6 +39,9 @@ using namespace kv_line;
 
 constexpr int EXTRA = 1; // units that an item's queries and result take besides
 constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32;
+constexpr float P_TOP = 14.f; // weights in f16 stay below 2^14
+// of k: the sum, relative to 2^(m + k - 14), holds 2^31 tokens.  Where all scales that a row sees are below 2^-80, f16's last bits go unused
+constexpr float K_MIN = -80.f, K_MAX = 121.f;
 static_assert(WARPS * STEP == UNIT, "a warp takes one step of each unit");
 
 // blocks per SM
@@ -75,6 +83,16 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// 2^n of a whole number -126 <= n <= 127
+__device__ __forceinline__ float pow2(float n) { return __uint_as_float(__float_as_uint(n + (8388608.f + 127.f)) << 23); }
+// to f16, at most its largest number: where scores are so large (2^25) that differences of them are whole numbers off
+__device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// a whole number above the base-2 logarithm of a value with these bits, by one at most
+__device__ __forceinline__ float above_log2(uint32_t bits) { return (float)((int)(bits >> 23) - 126); }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -319,11 +337,11 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         int all_see = 0x7fffffff; // up to this token no row of the item is masked
         if (rows > 0) all_see = s.first + (tile * ROWS) / group;
 
-        float o[MT][NB][4], m[NB][2], l[NB][2];
-        int ref = -200; // the values' common exponent
+        float o[MT][NB][4], m[NB][2], k2[NB][2], l[NB][2]; // k2: k
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             m[nb][0] = m[nb][1] = -INFINITY;
+            k2[nb][0] = k2[nb][1] = K_MIN;
             l[nb][0] = l[nb][1] = 0.f;
 #pragma unroll
             for (int i = 0; i < MT; ++i) o[i][nb][0] = o[i][nb][1] = o[i][nb][2] = o[i][nb][3] = 0.f;
@@ -383,8 +401,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             float top[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                top[nb][0] = m[nb][0];
-                top[nb][1] = m[nb][1];
+                top[nb][0] = top[nb][1] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -408,35 +425,63 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) top[nb][h] = fmaxf(top[nb][h], st[i >> 1][nb][(i & 1) * 2 + h]);
-            bool grew = false;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int w = 4; w < 32; w <<= 1) top[nb][h] = fmaxf(top[nb][h], __shfl_xor_sync(~0u, top[nb][h], w));
-                    grew |= top[nb][h] > m[nb][h];
-                }
             cp_wait<2 * S::STAGES - 1>();
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 4; ++i) vs[i] = sv[g + 8 * i];
-            // the largest value scale's exponent (scales are not negative, so their bits compare like them)
-            const uint32_t vmax = __reduce_max_sync(~0u, max(max(__float_as_uint(vs[0]), __float_as_uint(vs[1])),
-                                                                 max(__float_as_uint(vs[2]), __float_as_uint(vs[3]))));
-            const int e = max(ref, min(max((int)(vmax >> 23) - 126, -120), 126));
-            if (__any_sync(~0u, grew) || e > ref) {
-                const float f = ref <= -200 ? 0.f : __uint_as_float((uint32_t)max(127 + ref - e, 0) << 23);
-                ref = e;
+            // the largest and the smallest value scale (scales are positive, so their bits compare like them; 0: no such token)
+            uint32_t vb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vb[i] = __float_as_uint(vs[i]);
+            const uint32_t vmax = __reduce_max_sync(~0u, max(max(vb[0], vb[1]), max(vb[2], vb[3])));
+            const uint32_t vmin = __reduce_min_sync(~0u, min(min(vb[0] - 1, vb[1] - 1), min(vb[2] - 1, vb[3] - 1)));
+            // `now`: the largest score with this step; `rel`: the largest x + log2(scale) of the step's tokens, or up to 5 more,
+            // less `now` (differences first, so that scores of any size keep them)
+            float now[NB][2], rel[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    now[nb][h] = fmaxf(m[nb][h], top[nb][h]);
+                    rel[nb][h] = (top[nb][h] - now[nb][h]) + above_log2(vmax);
+                }
+            if (vmax > 0 && (vmax >> 23) > (vmin >> 23) + 4) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float &y = rel[nb][h];
+                        y = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y = fmaxf(y, (st[i >> 1][nb][(i & 1) * 2 + h] - now[nb][h]) + above_log2(vb[i]));
+#pragma unroll
+                        for (int w = 4; w < 32; w <<= 1) y = fmaxf(y, __shfl_xor_sync(~0u, y, w));
+                    }
+            }
+            bool grew = false;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) grew |= now[nb][h] > m[nb][h] || rel[nb][h] > k2[nb][h];
+            if (__any_sync(~0u, grew)) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     float fo[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float d = top[nb][h] == -INFINITY ? 1.f : ex2(m[nb][h] - top[nb][h]);
-                        l[nb][h] *= d;
-                        fo[h] = d * f;
-                        m[nb][h] = top[nb][h];
+                        // (fmaxf passes over the NaN of infinite scores, or of none)
+                        const float less = m[nb][h] - now[nb][h];
+                        const float k = fminf(fmaxf(fmaxf(k2[nb][h] + ceilf(less), ceilf(rel[nb][h])), K_MIN), K_MAX);
+                        fo[h] = now[nb][h] == -INFINITY ? 1.f : ex2(less + (k2[nb][h] - k));
+                        l[nb][h] *= fo[h];
+                        m[nb][h] = now[nb][h];
+                        k2[nb][h] = k;
                     }
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
@@ -447,9 +492,6 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                     }
                 }
             }
-            const float down = __uint_as_float((uint32_t)(127 - ref) << 23);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vs[i] *= down;
 
             // ---- weights, and the weighted values
 #pragma unroll
@@ -457,18 +499,19 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                 uint32_t pb[NB][2], rest[NB][2];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+                    const float m0 = (m[nb][0] == -INFINITY ? 0.f : m[nb][0]) + (k2[nb][0] - P_TOP);
+                    const float m1 = (m[nb][1] == -INFINITY ? 0.f : m[nb][1]) + (k2[nb][1] - P_TOP);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float w0 = ex2(st[tt][nb][i * 2] - m0), w1 = ex2(st[tt][nb][i * 2 + 1] - m1);
                         l[nb][0] += w0;
                         l[nb][1] += w1;
                         const float p0 = w0 * vs[tt * 2 + i], p1 = w1 * vs[tt * 2 + i];
-                        const uint32_t hi = pack_f16x2(p0, p1);
+                        const uint32_t hi = pack_held_f16x2(p0, p1);
                         pb[nb][i] = transposed(hi);
                         if (FINE) {
                             const float2 had = f16x2_to_f32(hi);
-                            rest[nb][i] = transposed(pack_f16x2(p0 - had.x, p1 - had.y));
+                            rest[nb][i] = transposed(pack_held_f16x2(p0 - had.x, p1 - had.y));
                         }
                     }
                 }
@@ -515,13 +558,15 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
 
         // ---- the four warps' parts together
         float *mine = (float *)ring;
-        const float up = ref <= -200 ? 0.f : __uint_as_float((uint32_t)(127 + ref) << 23);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
+            const float up[2] = { // from here on relative to 2^m
+                    pow2(k2[nb][0] - P_TOP), pow2(k2[nb][1] - P_TOP)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) l[nb][h] += __shfl_xor_sync(~0u, l[nb][h], w);
+                l[nb][h] *= up[h];
                 // a NaN among the scores, which no maximum shows, is to be the row's result
                 if (l[nb][h] != l[nb][h]) m[nb][h] = INFINITY;
                 if (g == 0) merge_m[warp][nb * 8 + 2 * t + h] = m[nb][h], merge_l[warp][nb * 8 + 2 * t + h] = l[nb][h];
@@ -532,7 +577,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                 const int d = DP == 64 ? g * 8 + i * 2 : (i >> 3) * 128 + g * 16 + (i & 7) * 2;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    *(float2 *)(mine + (nb * 8 + 2 * t + h) * S::PITCH + d) = make_float2(o[i][nb][h] * up, o[i][nb][2 + h] * up);
+                    *(float2 *)(mine + (nb * 8 + 2 * t + h) * S::PITCH + d) = make_float2(o[i][nb][h] * up[h], o[i][nb][2 + h] * up[h]);
             }
         }
         __syncthreads();

@@ -60,3 +60,127 @@ def test_a_sequence_of_two_thousand_million_tokens(gpu, impl, news, length):
     else:
         s.wait()
     assert ((dst[:, 0].double() - want).abs() <= size * 2.0 ** -4).all()
+
+
+# ---- what a row may not depend on, and how closely it is kept --------------------------------------------------
+
+def by_row(c, q, scale, weights=None):
+    """(result, sum of p |v|, largest p * value scale * peak, tokens) of every row in 64 bits, the middle two relative to the sum
+    of p, over the tokens that the row sees and no others; and the largest sum of |q| |k| that a score has.
+    `weights`: what p * value scale (relative to the largest of the row) is rounded to before the product."""
+    torch, _ = T._torch()
+    group = q.shape[1] // c.heads
+    want, size, most = (torch.zeros(q.shape[:2] + (n,), dtype=torch.float64, device="cuda") for n in (c.dim, c.dim, 1))
+    tokens, reach = torch.zeros(q.shape[0], 1, 1, dtype=torch.float64, device="cuda"), 0.0
+    for b, (n, length) in enumerate(zip(c.news, c.lens)):
+        lo = int(c.np_off[b])
+        idx = torch.from_numpy(c.np_table[b, :-(-length // c.page)].astype(np.int64)).cuda()
+        unit = c.scales[1][idx].double().T.repeat_interleave(c.page, 1)[:, :length].repeat_interleave(group, 0)[:, None]  # (heads, 1, tokens)
+        k, v = (c.dense(w, b, length).repeat_interleave(group, 1).transpose(0, 1) for w in (0, 1))
+        x = q[lo:lo + n].double().transpose(0, 1)
+        at = length - n + torch.arange(n, device="cuda")
+        hidden = (torch.arange(length, device="cuda")[None] > at[:, None])[None]
+        z = (x @ k.transpose(1, 2) * scale).masked_fill(hidden, -math.inf)
+        reach = max(reach, float((x.abs() @ k.abs().transpose(1, 2) * abs(scale)).masked_fill(hidden, 0).max()))
+        p = torch.exp(z - z.amax(-1, keepdim=True))
+        total = p.sum(-1, keepdim=True)
+        pv = p * unit
+        top = pv.amax(-1, keepdim=True)
+        if weights is not None:
+            pv = weights(pv / top) * top
+        code = v / unit.transpose(1, 2)
+        want[lo:lo + n] = (pv @ code / total).transpose(0, 1)
+        size[lo:lo + n] = (p @ v.abs() / total).transpose(0, 1)
+        most[lo:lo + n] = (top / total * T.PEAK[c.kind]).transpose(0, 1)
+        tokens[lo:lo + n] = at[:, None, None].double() + 1
+    return want, size, most, tokens, reach
+
+
+def closeness(c, q, scale, kind):
+    """Off by at most (all of it over the tokens that the row sees): the weights' rounding, 2^-11 of each where the result is
+    bf16, 2^-11 of what that left where it is f16 (2^-22), and half f16's smallest step, 2^-25, where the row's largest weight
+    is kept at 2^-1 or above: 2^-24 of that per token; logarithm and exponential of the value scales 2^-21 together; a score's
+    error, as in check_attention, twice; sums of `tokens` / 16 instructions' results, 2^-22 each; half a step of the result."""
+    want, size, most, tokens, reach = by_row(c, q, scale)
+    score = (c.dim + 8) * 2.0 ** -22 * reach + 64 * T.U
+    weight = 2.0 ** -11 if kind == "bf16" else 2.0 ** -22
+    tol = size * (weight + 2.0 ** -21 + 2 * score + (tokens / 16 + 4) * 2.0 ** -22) + most * tokens * 2.0 ** -24
+    return want, tol + want.abs() * T.HALF[kind] + (2.0 ** -25 if kind == "f16" else 2.0 ** -134)
+
+
+# (lens, news, page): the newest tokens lie in several pages, so that rows of one tile see different ones
+SPREAD = {"step": ([700, 33, 256], [1, 1, 1], 16), "draft": ([64, 131, 40], [9, 7, 11], 8), "uneven": ([90, 45], [8, 20], 5),
+          "prompt": ([400, 300], [200, 300], 32), "runs of 8": ([300, 129], [150, 129], 24)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, GENERIC])
+@pytest.mark.parametrize("kind", ["s8", "e4m3"])
+@pytest.mark.parametrize("shape", list(SPREAD))
+@pytest.mark.parametrize("what", ["last page large", "every other page large", "large pages without weight", "first page small",
+                                  "first pages of zeros", "zeros everywhere else", "rising", "all small", "all large"])
+def test_value_scales_of_pages_that_do_not_count(gpu, impl, kind, shape, what):
+    """Pages whose values are 2^20 .. 2^60 times the others', which rows do not see, or give no weight, or do: every row is
+    held to what it sees itself."""
+    torch, _ = T._torch()
+    lens, news, page = SPREAD[shape]
+    for dim, power in ((128, 24), (64, 40), (80, 60)):
+        c = Cache(lens, news, 2, page, dim, kind, seed=power)
+        q = torch.randn(c.rows, 8, dim, generator=c.g, device="cuda")
+        big = 2.0 ** power
+        for b, n in enumerate(lens):
+            ids = torch.from_numpy(c.np_table[b, :-(-n // page)].astype(np.int64)).cuda()
+            v = c.scales[1]
+            if what == "last page large":
+                v[ids[-1]] *= big
+            elif what == "every other page large":
+                v[ids[::2]] *= big
+            elif what == "large pages without weight":
+                # scores of some -100 there, of some 0 elsewhere: weights of 2^-144, values of 2^power
+                q = q.abs()
+                c.codes[0].view(torch.int8)[ids[1::3]] = -64 if kind == "s8" else -0x80 + 0x68  # -64, both
+                c.scales[0][ids[1::3]] = 100 / (64 * 0.1 * 0.79 * dim)
+                v[ids[1::3]] *= big
+            elif what == "first page small":
+                v[ids[0]] /= big
+            elif what == "first pages of zeros":
+                for w in (0, 1):
+                    c.codes[w][ids[:2]] = 0
+                    c.scales[w][ids[:2]] = T.TINY
+            elif what == "zeros everywhere else":
+                c.codes[1][ids[::2]] = 0
+                v[ids[::2]] = T.TINY
+            elif what == "rising":
+                v[ids] *= torch.exp2(torch.linspace(-power, 10, len(ids), device="cuda")).floor()[:, None].clamp_min(2.0 ** -power)
+            elif what == "all small":
+                v[ids] /= big
+            else:
+                v[ids] *= big
+        q = q.to(torch.bfloat16)
+        dst = torch.full_like(q, math.nan)
+        run_attention(gpu, c, q, dst, 0.1, impl)
+        gpu[1].wait()
+        want, tol = closeness(c, q, 0.1, "bf16")
+        err = (dst.double() - want).abs()
+        assert not torch.isnan(dst).any()
+        assert (err <= tol).all(), "%s: %g of the tolerance" % (power, float((err / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, GENERIC])
+@pytest.mark.parametrize("kind", ["s8", "e4m3"])
+@pytest.mark.parametrize("page", [16, 24])
+def test_f16_results_come_from_unrounded_weights(gpu, impl, kind, page):
+    """What is left of a weight after its rounding to f16 counts where the result is f16.  The allowance is small enough to tell:
+    the definition with weights rounded to f16 does not meet it."""
+    torch, _ = T._torch()
+    c = Cache([70, 96], [60, 90], 1, page, 128, kind, seed=page)
+    q = torch.randn(c.rows, 2, 128, generator=c.g, device="cuda").to(torch.float16)
+    scale = 0.002  # scores around 0.01, so that their own errors stay below 2^-18
+    dst = torch.full_like(q, math.nan)
+    run_attention(gpu, c, q, dst, scale, impl)
+    gpu[1].wait()
+    want, tol = closeness(c, q, scale, "f16")
+    assert ((dst.double() - want).abs() <= tol).all(), "%g of the tolerance" % float(((dst.double() - want).abs() / tol).max())
+    rounded = by_row(c, q, scale, weights=lambda w: (w * 8192).half().double() / 8192)[0].to(torch.float16)
+    assert ((rounded.double() - want).abs() > tol).any()
