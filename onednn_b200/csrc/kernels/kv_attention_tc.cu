@@ -18,14 +18,16 @@
 //   warp 14          finds the block's items ahead of all others and lays them out in shared memory
 //
 // The two scales stay out of the products.  A page holds a multiple of RUN (16 or 8) tokens here, so as many neighbouring tokens
-// share theirs: x = s * (key scale * softmax scale), and the value scale enters the exponent,
-// P = 2^(x - m + log2(value scale) - ref), so neither costs an operation per element; the sum takes P back by a
-// factor per run.  P is f16 relative to 2^8 (m follows the maximum only when that has grown by more, which saves
-// most rescaling of O) and to `ref`, a power of two above all value scales.  FINE (f16 results): what P's rounding left
-// is multiplied too.
+// share theirs: x = s * (key scale * softmax scale) in the exponent's multiply-add, P = w * value scale with
+// w = 2^(x - m - k + 14), two elements at a time, and the sum is of the w.  m and k are the row's own: m follows the largest
+// score that the row has seen when that has grown by more than 2^8, which saves most rescaling of O; k, a whole number, is
+// not below x + log2(value scale) - m of any token that the row sees.  So P < 2^14, rounded to f16 relative to what the row
+// sees, and no page that it does not see, or gives no weight, takes bits from the others (with the value scale in the
+// exponent, relative to the largest of all pages, 3 % faster, a page 2^30 above the others took them to zero in rows that
+// did not see it).  FINE (f16 results): what P's rounding left is multiplied too.
 //
 // Measured on one B200: three sequences with 1450, 1029 and 1710 new tokens on 5750, 4647 and 3543, 32 query heads on 8, dim 128, s8,
-// bf16: 328 us, 806 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
+// bf16: 340 us, 778 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
 // alone take 1.3.  What is left: a softmax step of 64 columns takes a warp 2000 cycles, two of the three warps on a
 // scheduler; items begin and end (8 us each) and cut ones are joined (10 us).  Not kept: 16 softmax warps, two threads per row
 // (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
@@ -62,12 +64,14 @@ struct smem_t {
 // The scales of a tile's tokens, run by run, as the softmax takes them.  Four tiles deep: the converters are at most
 // two ahead of the slower softmax.
 struct scales_t {
-    // x key scale, y 0 (-inf: no such page), z log2(value scale) - ref (-inf: no such page), w 2^-z
+    // x key scale, y 0 (-inf: no such page), z a whole number above log2(value scale), by one at most, w value scale
     float4 chunk[UNIT / 8];
-    float step; // what O is to be multiplied by: 2^(last tile's ref - this one's)
-    float up;   // 2^ref
+    float above, below; // whole numbers, not below and not above any log2(value scale)
 };
-
+constexpr float P_TOP = 14.f; // P stays below 2^14
+constexpr float ROOM = 8.f;   // what m, and with it k, may lag behind
+// of k: the sum, relative to 2^(m + k - 14), holds 2^31 tokens.  Where all scales that a row sees are below 2^-70, f16's last bits go unused
+constexpr float K_MIN = -70.f, K_MAX = 121.f;
 constexpr float SMALL = 1.0842022e-19f; // 2^-63
 
 // a stretch of an item's tokens: what one block does of it
@@ -225,11 +229,14 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-__device__ __forceinline__ float lg2(float x) {
-    float r;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+// to f16, at most its largest number: where scores are so large (2^25) that differences of them are whole numbers off
+__device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// 2^n of a whole number -126 <= n <= 127
+__device__ __forceinline__ float pow2(float n) { return __uint_as_float(__float_as_uint(n + (8388608.f + 127.f)) << 23); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -249,6 +256,11 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -423,7 +435,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
         while (seg && seg->rows > 0) {
             const int u0 = seg->u0, u1 = seg->u1;
             const bool active = ok && seg->rows > t * TILE, mine = t * TILE + r < seg->rows;
-            float m = -INFINITY, l = 0.f, up = 0.f; // up: 2^ref
+            float m = -INFINITY, k2 = K_MIN, l = 0.f; // k2: k; the largest of the warp's
             // the next segment: its queries come while this one's last tile is worked on, once that one's scores are there
             const segment_t *next = nullptr;
             float factor_next = 0.f;
@@ -454,8 +466,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     float4 ck[STEP / RUN];
 #pragma unroll
                     for (int k = 0; k < STEP / RUN; ++k) ck[k] = chunk[k];
-                    const float step = place == 0 ? sc.step : 1.f;
-                    up = sc.up;
                     tmem_ld32_issue(tmem_p, v[0]);
                     tmem_ld32_issue(tmem_p + 32, v[1]);
                     tmem_ld32_wait(v[0]);
@@ -466,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         for (int i = 0; i < STEP; ++i)
                             if (i > seen) v[i >> 5][i & 31] = 0xff800000u;
                     }
-                    float f[STEP / RUN], top = m;
+                    float f[STEP / RUN], xk[STEP / RUN], top = -INFINITY;
 #pragma unroll
                     for (int k = 0; k < STEP / RUN; ++k) {
                         const uint32_t *y = v[k * RUN >> 5] + (k * RUN & 31);
@@ -479,14 +489,30 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         }
                         x0 = max3(x0, x1, __uint_as_float(y[RUN / 2 - 1]));
                         f[k] = ck[k].x * factor;
-                        top = fmaxf(top, fmaf(fmaxf(x0, __uint_as_float(y[RUN - 1])), f[k], ck[k].y));
+                        xk[k] = fmaf(fmaxf(x0, __uint_as_float(y[RUN - 1])), f[k], ck[k].y);
+                        top = fmaxf(top, xk[k]);
                     }
-                    // ---- m and ref follow, seldom; O and the sum with them
-                    const bool follow = top > m + 8.f; // also from -inf
-                    if (__any_sync(~0u, follow || step != 1.f)) {
-                        const float d = follow ? ex2(m - top) : 1.f, fo = d * step;
-                        if (follow) m = top;
-                        l *= d;
+                    // ---- m and k follow, seldom; O and the sum with them.  `rel`: the largest x + log2(value scale) of the step, less
+                    // m (differences first, so that scores of any size keep them).  Runs of 8, twice as many, are looked at one by
+                    // one where their scales are further than 2^4 apart, else the largest stands for all (24 tokens per page: 345 us, each
+                    // time 350; with runs of 16 the branch costs as much as it saves: 340, without 338)
+                    const float from = m == -INFINITY ? top : m;
+                    float rel = (top - from) + sc.above;
+                    if (RUN == 16 || sc.above - sc.below > 5.f) {
+                        rel = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < STEP / RUN; ++k) rel = fmaxf(rel, (xk[k] - from) + ck[k].z);
+                    }
+                    const bool follow = top > m + ROOM || rel > k2; // also from -inf
+                    if (__any_sync(~0u, follow)) {
+                        float fo = 1.f;
+                        if (follow) { // (fmaxf passes over the NaN of infinite scores)
+                            const float now = fmaxf(m, top), less = m - now;
+                            const float k = fminf(fmaxf(fmaxf(k2 + ceilf(less), ceilf(rel + (from - now)) + ROOM), K_MIN), K_MAX);
+                            fo = ex2(less + (k2 - k));
+                            m = now, k2 = k;
+                        }
+                        l *= fo;
                         if (j > 0) { // the products of the step before are added up first
                             if (!(ok = products_done(place ^ 1))) break;
                             tc_fence_after();
@@ -501,15 +527,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         }
                     }
                     // ---- weights, over the scores: of each 16 columns the first eight, FINE: the other eight too
-                    const float base = m == -INFINITY ? 0.f : m;
+                    const float base = (m == -INFINITY ? 0.f : m) + (k2 - P_TOP);
 #pragma unroll
                     for (int h = 0; h < STEP / 16; ++h) {
                         uint32_t pw[FINE ? 16 : 8];
 #pragma unroll
                         for (int k = h * 16 / RUN; k < (h + 1) * 16 / RUN; ++k) {
                             const uint32_t *y = v[k * RUN >> 5] + (k * RUN & 31);
-                            const float off = ck[k].z - base;
-                            const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(off, off);
+                            const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(ck[k].y - base, ck[k].y - base), vv = f32x2(ck[k].w, ck[k].w);
                             uint64_t sum = 0;
 #pragma unroll
                             for (int i = 0; i < RUN; i += 2) {
@@ -517,15 +542,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                                 const float2 x = unpack2(fma2(f32x2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), ff, oo));
                                 const float e0 = ex2(x.x), e1 = ex2(x.y);
                                 sum = add2(sum, f32x2(e0, e1));
-                                const uint32_t hi = pack_f16x2(e0, e1);
+                                const float2 pv = unpack2(mul2(f32x2(e0, e1), vv));
+                                const uint32_t hi = pack_held_f16x2(pv.x, pv.y);
                                 pw[at] = hi;
                                 if (FINE) {
                                     const float2 had = f16x2_to_f32(hi);
-                                    pw[FINE ? 8 + at : 0] = pack_f16x2(e0 - had.x, e1 - had.y);
+                                    pw[FINE ? 8 + at : 0] = pack_held_f16x2(pv.x - had.x, pv.y - had.y);
                                 }
                             }
                             const float2 both = unpack2(sum);
-                            l = fmaf(both.x + both.y, ck[k].w, l);
+                            l += both.x + both.y;
                         }
                         if (FINE) tmem_st16(tmem_p + h * 16, pw);
                         else tmem_st8(tmem_p + h * 16, pw);
@@ -549,6 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
 
             // ---- the row's result, or its part of it
             const bool whole = seg->whole;
+            const float up = pow2(k2 - P_TOP); // O and l are relative to 2^(m + k - 14), parts to 2^m
             if (l != l) m = INFINITY; // a NaN among the scores, which no maximum shows
             const int idx = seg->row0 + t * TILE + r;
             char *to = (char *)p.dst + ((int64_t)(seg->begin + idx / group) * p.dst_s0 + ((int64_t)seg->head * group + idx % group) * p.dst_s1) * 2;
@@ -563,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                 store8(p.dst_dt, to + d * 2, y);
             };
             if (active && ok) {
-                const float inv = l == 0.f ? 0.f : up / l;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
                 for (int h = 0; h < DP / 32; ++h) {
                     uint32_t v[32];
@@ -586,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     __syncwarp(); // the next load is the whole warp's, lanes without a row among them
                 }
                 tc_fence_before(); // O may be written again after the next arrival
-                if (!whole && mine) part[pr] = m, part[ROWS + pr] = l;
+                if (!whole && mine) part[pr] = m, part[ROWS + pr] = l * up;
             }
             if (!whole && ok) {
                 // an item in several parts: the last block to finish one puts them together, in the order of the parts
@@ -663,7 +690,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
             give_back(seg_i++);
             const uint8_t *keys = (const uint8_t *)c.key + head * c.s_head + cc * 16, *values = (const uint8_t *)c.value + head * c.s_head + cc * 16;
             uint4 kr[LOADS], vr[LOADS];
-            // every warp looks up all runs of a tile, one per lane, because `ref` needs all their scales
+            // every warp looks up all runs of a tile, one per lane
             int64_t place = -1;
             float ks = -1.f, vs = 0.f;
             int n = (u0 * UNIT + lane * RUN) / page, slot = u0 * UNIT + lane * RUN - n * page;
@@ -715,28 +742,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     *(uint4 *)(to + piece_at(row, cc * 2 + 1)) = make_uint4(d.x, d.y, e.x, e.y);
                 }
             };
-            float ref = -200.f;
             // keys of unit j (the i-th since the launch), and both scales: a softmax that sees the scores sees them
             auto put_keys = [&](uint32_t i) {
                 const int st = i % STAGES;
                 const uint32_t use = i / STAGES;
                 if (use > 0 && !(ok = warp_wait(&ctrl->k_empty[st], (use - 1) & 1, ctrl, status))) return;
-                const float log = lg2(fmaxf(vs, 7.5231638e-37f)); // 2^-120 at least
-                float top = lane < CHUNKS ? log : -200.f;
-#pragma unroll
-                for (int o = CHUNKS / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-                top = __shfl_sync(~0u, top, 0);
-                // with room, so that it seldom moves
-                const float now = top > ref ? ceilf(top) + 1.f : ref;
-                if (w == 0 && lane < CHUNKS) {
-                    scales_t &sc = ctrl->scales[i & 3];
+                if (w == 0) {
                     const bool there = ks >= 0.f;
-                    // scales below 2^-60 of the largest count as that: their values round to nothing, their weights stay in the sum
-                    const float z = fmaxf(log - now, -60.f);
-                    sc.chunk[lane] = make_float4(fmaxf(ks, SMALL), there ? 0.f : -INFINITY, there ? z : -INFINITY, ex2(-z));
-                    if (lane == 0) sc.step = now == ref ? 1.f : ex2(ref - now), sc.up = ex2(now);
+                    // scales are positive, so their bits compare like them
+                    const uint32_t bits = __float_as_uint(vs), vmax = __reduce_max_sync(~0u, there ? bits : 0u);
+                    const uint32_t vmin = min(__reduce_min_sync(~0u, there ? bits : ~0u), vmax);
+                    scales_t &sc = ctrl->scales[i & 3];
+                    const float above = (float)((int)(bits >> 23) - 126);
+                    if (lane < CHUNKS) sc.chunk[lane] = there ? make_float4(fmaxf(ks, SMALL), 0.f, above, vs) : make_float4(SMALL, -INFINITY, 0.f, 0.f);
+                    if (lane == 0) sc.above = (float)((int)(vmax >> 23) - 126), sc.below = (float)((int)(vmin >> 23) - 127);
                 }
-                ref = now;
                 convert(kr, smem_k + st * S::MAT);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();

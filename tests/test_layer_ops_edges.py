@@ -114,7 +114,7 @@ SPREAD = {"step": ([700, 33, 256], [1, 1, 1], 16), "draft": ([64, 131, 40], [9, 
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("impl", [MMA, GENERIC])
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
 @pytest.mark.parametrize("kind", ["s8", "e4m3"])
 @pytest.mark.parametrize("shape", list(SPREAD))
 @pytest.mark.parametrize("what", ["last page large", "every other page large", "large pages without weight", "first page small",
@@ -167,7 +167,7 @@ def test_value_scales_of_pages_that_do_not_count(gpu, impl, kind, shape, what):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("impl", [MMA, GENERIC])
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
 @pytest.mark.parametrize("kind", ["s8", "e4m3"])
 @pytest.mark.parametrize("page", [16, 24])
 def test_f16_results_come_from_unrounded_weights(gpu, impl, kind, page):
