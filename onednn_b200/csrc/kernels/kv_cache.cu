@@ -196,7 +196,8 @@ __device__ __forceinline__ void read_row(const b200_kv_rows_params_t &p, const s
         phys = page_of(c, b, at, slot);
         if (phys < 0 && lane == 0) flag_bad_page(c);
     }
-    const int unit = VEC ? 16 : 1, per = (int)c.dim / unit, all = per * (int)c.heads, esize = dt_bits(p.dt) / 8;
+    const int unit = VEC ? 16 : 1, esize = dt_bits(p.dt) / 8;
+    const uint32_t per = (uint32_t)c.dim / unit, all = per * (uint32_t)c.heads; // 2^30 at most: twice that, and the step behind it, fit
     const int64_t place = (int64_t)phys * c.s_page + (int64_t)slot * c.s_slot;
     auto put = [&](char *d, const uint4 &w, float scale) {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -210,9 +211,9 @@ __device__ __forceinline__ void read_row(const b200_kv_rows_params_t &p, const s
             store8(p.dt, d + 8 * j * esize, v);
         }
     };
-    for (int i = lane; i < 2 * all; i += 32) {
+    for (uint32_t i = lane; i < 2 * all; i += 32) {
         const bool val = i >= all;
-        const int k = val ? i - all : i, head = k / per, e = (k - head * per) * unit;
+        const uint32_t k = val ? i - all : i, head = k / per, e = (k - head * per) * unit;
         char *d = (char *)(val ? p.value : p.key) + (row * p.s_row + head * p.s_head + e) * esize;
         const uint8_t *from = (const uint8_t *)(val ? c.value : c.key) + place + head * c.s_head + e;
         const float scale = phys < 0 ? 0.f : (val ? c.value_scale : c.key_scale)[(int64_t)phys * c.heads + head];

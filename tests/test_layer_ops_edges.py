@@ -184,3 +184,37 @@ def test_f16_results_come_from_unrounded_weights(gpu, impl, kind, page):
     assert ((dst.double() - want).abs() <= tol).all(), "%g of the tolerance" % float(((dst.double() - want).abs() / tol).max())
     rounded = by_row(c, q, scale, weights=lambda w: (w * 8192).half().double() / 8192)[0].to(torch.float16)
     assert ((rounded.double() - want).abs() > tol).any()
+
+
+@pytest.mark.gpu
+def test_a_token_of_two_to_the_thirty_elements(gpu):
+    """2^30 - 1 in all heads together, next to the largest that the descriptors take, element by element."""
+    torch, _ = T._torch()
+    heads, dim = 32767, 32769
+    e, s = gpu
+    n = heads * dim
+    buf = [torch.randint(-127, 128, (n + 1,), dtype=torch.int8, device="cuda") for _ in range(2)]
+    c = Cache([1], [1], 1, 1, 16, "s8", spare=0)
+    c.codes = [b[1:].view(1, heads, 1, dim) for b in buf]
+    c.scales = [torch.rand(1, heads, device="cuda") + 0.5 for _ in range(2)]
+    out = [torch.full((1 + n,), 9, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    k, v = (o[1:].view(1, heads, dim) for o in out)
+    p = api.Primitive(api.kv_cache_read_primitive_desc(e, tmd(c.codes[0]), tmd(k), tmd(c.table)))
+    p.execute(s, {**c.args(e), api.ARG_DST: mem(k, e), api.ARG_DST_1: mem(v, e)})
+    s.wait()
+    assert all(float(o[0]) == 9 for o in out)
+    for i, got in enumerate((k, v)):
+        for h in range(0, heads, 256):
+            want = (c.codes[i][0, h:h + 256, 0].float() * c.scales[i][0, h:h + 256, None]).to(torch.bfloat16)
+            assert torch.equal(got[0, h:h + 256], want)
+    # and appended: the same codes again, from values that they stand for
+    x = [(c.codes[i][:, :, 0].to(torch.bfloat16)) for i in range(2)]
+    for i in range(2):
+        x[i][:, :, 0] = 127  # every head's scale is 127 / 127
+    c.codes = [torch.zeros_like(t) for t in c.codes]
+    run_append(gpu, c, x[0], x[1])
+    s.wait()
+    one = (torch.full((), 127.0) * torch.tensor(1 / 127.0)).item()  # in f32
+    for i in range(2):
+        assert (c.scales[i] == one).all()
+        assert torch.equal(c.codes[i][:, :, 0], x[i].to(torch.int8))
