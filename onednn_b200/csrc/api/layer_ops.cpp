@@ -131,6 +131,27 @@ void *at(const std::map<int, dnnl_memory *> &args, int arg) {
     return (char *)it->second->handle + md.offset0 * dt_nbits(md.data_type) / 8;
 }
 
+// Whether two tensors of one descriptor, `d` elements apart, have an element in common: d is a sum of whole multiples of the
+// strides, each of fewer than the dim's size.  Strides are nested (the descriptor's creation has checked), so for each from
+// the largest on only the two multiples next to what is left can do.
+bool overlap(const dnnl_memory_desc &md, int64_t d, uint32_t done = 0) {
+    int big = -1;
+    for (int i = 0; i < md.ndims; ++i)
+        if (!(done >> i & 1) && md.dims[i] > 1 && (big < 0 || md.strides[i] > md.strides[big])) big = i;
+    if (big < 0) return d == 0;
+    const int64_t s = md.strides[big], n = md.dims[big], q = d / s - (d % s < 0);
+    for (const int64_t k : {q, q + 1})
+        if (k > -n && k < n && overlap(md, d - k * s, done | 1u << big)) return true;
+    return false;
+}
+// the same for two arguments; neither empty.  (What begins inside an element of the other's has been refused where elements
+// have to be aligned; 8-bit ones always are.)
+bool overlap(const std::map<int, dnnl_memory *> &args, int one, int other) {
+    const dnnl_memory_desc &md = args.at(one)->md;
+    const int64_t bytes = (char *)at(args, other) - (char *)at(args, one);
+    return overlap(md, bytes / (dt_nbits(md.data_type) / 8));
+}
+
 dnnl_status_t status_of(int rc) {
     if (rc == 0) return dnnl_success;
     if (rc == B200_ERR_UNSUPPORTED || rc == B200_ERR_TOO_LARGE) return dnnl_unimplemented;
@@ -349,11 +370,14 @@ dnnl_status_t ext_execute(const dnnl_primitive *prim, dnnl_stream *stream, const
         // no element may straddle its type's boundary: a kernel that read it would fault
         if ((uintptr_t)it->second->handle % (dt_nbits(want.second.data_type) / 8) != 0) return dnnl_invalid_arguments;
     }
-    // blocks of the append write keys and values side by side: in one place they would race
-    if (pd->kind == dnnl_b200_kv_cache_append
-            && (at(args, DNNL_ARG_B200_KEY_SCALES) == at(args, DNNL_ARG_B200_VALUE_SCALES)
-                    || at(args, DNNL_ARG_B200_KEY_CACHE) == at(args, DNNL_ARG_B200_VALUE_CACHE))
-            && !pd->dst.has_zero_dim())
+    // keys and values are written side by side: in places that they share they would race
+    if (pd->kind == dnnl_b200_kv_cache_append && !pd->dst.has_zero_dim()
+            && (overlap(args, DNNL_ARG_B200_KEY_SCALES, DNNL_ARG_B200_VALUE_SCALES)
+                    || overlap(args, DNNL_ARG_B200_KEY_CACHE, DNNL_ARG_B200_VALUE_CACHE)))
+        return dnnl_invalid_arguments;
+    if (pd->kind == dnnl_b200_kv_cache_read && overlap(args, DNNL_ARG_DST, DNNL_ARG_DST_1)) return dnnl_invalid_arguments;
+    // and a row's result would be written over its sum
+    if (pd->kind == dnnl_b200_rms_norm && pd->ext_args.count(DNNL_ARG_DST_1) && at(args, DNNL_ARG_DST) == at(args, DNNL_ARG_DST_1))
         return dnnl_invalid_arguments;
     switch (pd->kind) {
         case dnnl_b200_rms_norm: return norm_execute(pd, stream, args);

@@ -218,3 +218,69 @@ def test_a_token_of_two_to_the_thirty_elements(gpu):
     for i in range(2):
         assert (c.scales[i] == one).all()
         assert torch.equal(c.codes[i][:, :, 0], x[i].to(torch.int8))
+
+
+# ---- buffers that lie in one another ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+def test_outputs_that_share_places_are_refused(gpu):
+    """Keys' and values' caches, scales or rows that share elements without being the same memory; ones that lie in each
+    other's gaps are taken."""
+    torch, _ = T._torch()
+    e, s = gpu
+    heads, page, dim = 2, 16, 32
+    c = Cache([20, 3], [2, 3], heads, page, dim, "s8")
+    x = torch.randn(c.rows, heads, dim, generator=c.g, device="cuda")
+    both = torch.zeros(2 * c.pages, heads, page, 2, dim, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(2 * c.pages, heads, device="cuda")
+    rows = torch.zeros(64, heads, 2, dim, device="cuda")
+
+    def cache_at(first):
+        return api.Memory(tmd(both[:c.pages, :, :, 0]), e, both.data_ptr() + first)
+
+    def append(key_at, value_at, key_scale=0, value_scale=c.pages * heads):
+        f32 = tmd(scales[:c.pages])
+        p = api.Primitive(api.kv_cache_append_primitive_desc(e, tmd(x), tmd(both[:c.pages, :, :, 0]), tmd(c.table)))
+        p.execute(s, {**c.args(e), api.ARG_SRC: mem(x, e), api.ARG_SRC_1: mem(x, e), api.ARG_B200_KEY_CACHE: cache_at(key_at),
+                      api.ARG_B200_VALUE_CACHE: cache_at(value_at), api.ARG_B200_KEY_SCALES: api.Memory(f32, e, scales.data_ptr() + 4 * key_scale),
+                      api.ARG_B200_VALUE_SCALES: api.Memory(f32, e, scales.data_ptr() + 4 * value_scale)})
+
+    def refused(f, *a):
+        with pytest.raises(api.Error) as err:
+            f(*a)
+        assert err.value.name == "invalid_arguments"
+    slot, head = 2 * dim, 2 * dim * page
+    one = head * heads  # bytes of a page
+    for a, b in ((0, 0), (0, 1), (0, dim - 1), (0, slot), (5 * slot, 0), (0, head), (0, one), (0, (c.pages - 1) * one + head), (one, 1), (0, slot + dim - 1),
+                 (0, head - slot + dim + 1)):
+        refused(append, a, b)
+    for a, b in ((0, 1), (heads, 0), (0, c.pages * heads - 1)):
+        refused(append, 0, dim, a, b)
+    s.wait()
+    assert not both.any() and not scales.any()
+    # values in the gaps between keys, and on the other side of them; behind one another
+    want = [T.expected_append(c, x, torch.zeros(c.pages, heads, page, dim, dtype=torch.int8, device="cuda"), scales[:c.pages])[0] for _ in range(2)]
+    for a, b in ((0, dim), (dim, 0), (0, c.pages * one), (0, c.pages * one + dim)):
+        both.zero_()
+        scales.zero_()
+        append(a, b)
+        s.wait()
+        flat = both.view(-1)
+        for at, w in ((a, want[0]), (b, want[1])):
+            got = flat.as_strided((c.pages, heads, page, dim), (one, head, slot, 1), at)
+            assert torch.equal(got, w)
+    p = api.Primitive(api.kv_cache_read_primitive_desc(e, tmd(c.codes[0]), tmd(rows[:5, :, 0]), tmd(c.table)))
+
+    def read(first, second):
+        d = tmd(rows[:5, :, 0])
+        p.execute(s, {**c.args(e), api.ARG_DST: api.Memory(d, e, rows.data_ptr() + 4 * first), api.ARG_DST_1: api.Memory(d, e, rows.data_ptr() + 4 * second)})
+    for a, b in ((0, 0), (0, 1), (2 * dim, 0), (0, 4 * heads * 2 * dim)):
+        refused(read, a, b)
+    for a, b in ((0, dim), (0, 5 * heads * 2 * dim)):
+        read(a, b)
+    s.wait()
+    r = torch.randn(4, 64, device="cuda")
+    h = torch.zeros_like(r)
+    norm = api.Primitive(api.rms_norm_primitive_desc(e, tmd(r), tmd(r), 1e-5, residual_md=tmd(r)))
+    refused(norm.execute, s, {api.ARG_SRC: mem(r, e), api.ARG_SRC_1: mem(r, e), api.ARG_DST: mem(h, e), api.ARG_DST_1: mem(h, e)})
+    s.wait()
