@@ -284,3 +284,147 @@ def test_outputs_that_share_places_are_refused(gpu):
     norm = api.Primitive(api.rms_norm_primitive_desc(e, tmd(r), tmd(r), 1e-5, residual_md=tmd(r)))
     refused(norm.execute, s, {api.ARG_SRC: mem(r, e), api.ARG_SRC_1: mem(r, e), api.ARG_DST: mem(h, e), api.ARG_DST_1: mem(h, e)})
     s.wait()
+
+
+# ---- batches and layouts ---------------------------------------------------------------------------------------
+
+STEP = dict(lens=[700, 33, 256], news=[1, 1, 1], heads=2, page=16, dim=128, kind="s8")
+PROMPT = dict(lens=[700, 300], news=[200, 300], heads=2, page=32, dim=128, kind="s8")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
+def test_lengths_beyond_the_table_leave_exactly_the_tokens_that_it_holds(gpu, impl):
+    """Every row stands behind the table's end and sees all slots of the pages that the table names inside the cache; the
+    rest is left out and reported."""
+    torch, _ = T._torch()
+    e, s = gpu
+    spec = PROMPT if impl == TC else STEP
+    c = Cache(**spec, seed=11)
+    q = torch.randn(c.rows, 8, c.dim, generator=c.g, device="cuda").to(torch.bfloat16)
+    c.kv_lens += 100000
+    dst = torch.full_like(q, math.nan)
+    run_attention(gpu, c, q, dst, 0.1, impl)
+    T.bad_wait(s)
+    for b, n in enumerate(c.news):
+        rows = slice(int(c.np_off[b]), int(c.np_off[b]) + n)
+        pages = [int(v) for v in c.np_table[b] if 0 <= v < c.pages]
+        one = Cache([len(pages) * c.page], [n], c.heads, c.page, c.dim, c.kind)
+        one.codes, one.scales, one.np_table, one.pages = c.codes, c.scales, np.asarray([pages], dtype=np.int32), c.pages
+        k, v = (one.dense(w, 0, one.lens[0]).repeat_interleave(4, 1).transpose(0, 1) for w in (0, 1))
+        z = q[rows].double().transpose(0, 1) @ k.transpose(1, 2) * 0.1
+        reach = float((q[rows].double().abs().transpose(0, 1) @ k.abs().transpose(1, 2) * 0.1).max())
+        p = torch.softmax(z, -1)
+        want, size = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
+        # as in closeness(): weights, scores, sums, result, and 2^-24 of the largest value for each of up to 2^10 tokens
+        tol = size * (2.0 ** -11 + 2 * ((c.dim + 8) * 2.0 ** -22 * reach + 64 * T.U) + 64 * 2.0 ** -22) + want.abs() * 2.0 ** -8 + float(v.abs().max()) * 2.0 ** -14
+        assert ((dst[rows].double() - want).abs() <= tol).all()  # NaN, what was there before, does not pass
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
+@pytest.mark.parametrize("news", [[0, 0, 0], [1, 0, 1], [0, 40, 0]])
+def test_descriptors_larger_than_the_batch(gpu, impl, news):
+    """A primitive for 4096 rows takes batches of none, of a step, of a prompt piece; the rows behind stay."""
+    torch, types = T._torch()
+    c = Cache([90, 300, 17], news, 2, 16, 64, "e4m3", before=2, behind=4094 - sum(news), seed=3)
+    q = torch.randn(c.rows, 4, 64, generator=c.g, device="cuda").to(torch.bfloat16)
+    dst = torch.full_like(q, 3.0)
+    kept = dst.clone()
+    run_attention(gpu, c, q, dst, 0.1, impl)
+    gpu[1].wait()
+    check_attention(c, q, 0.1, dst, kept, "bf16")
+    x = torch.randn(c.rows, 2, 64, generator=c.g, device="cuda").to(torch.bfloat16)
+    want = [T.expected_append(c, x, c.codes[i], c.scales[i]) for i in range(2)]
+    run_append(gpu, c, x, x)
+    gpu[1].wait()
+    for i in range(2):
+        assert torch.equal(c.scales[i], want[i][1]) and torch.equal(c.codes[i].contiguous().view(torch.int8), want[i][0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
+@pytest.mark.parametrize("lens,news,page,dim", [([130, 61], [100, 61], 16, 64), ([40, 97], [1, 2], 1, 64), ([75, 20], [3, 20], 24, 128)])
+def test_token_major_pages_and_head_major_rows(gpu, impl, lens, news, page, dim):
+    """Other orders of the same dims: pages (token, head, dim) in memory, queries and results (head, row, dim), a table with rows
+    wider than its columns."""
+    torch, types = T._torch()
+    e, s = gpu
+    c = Cache(lens, news, 2, page, dim, "s8", seed=page)
+    c.codes = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in c.codes]
+    wide = torch.full((len(lens), c.table.shape[1] + 3), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c.table.shape[1]] = c.table
+    c.table = wide[:, :c.table.shape[1]]
+    x = torch.randn(2, c.rows, dim, generator=c.g, device="cuda").to(torch.float16).transpose(0, 1)  # (rows, heads, dim), head-major
+    want = [T.expected_append(c, x, c.codes[i], c.scales[i]) for i in range(2)]
+    run_append(gpu, c, x, x)
+    s.wait()
+    for i in range(2):
+        assert torch.equal(c.scales[i], want[i][1]) and torch.equal(c.codes[i].contiguous(), want[i][0])
+    q = torch.randn(8, c.rows, dim, generator=c.g, device="cuda").to(torch.bfloat16).transpose(0, 1)
+    dst = torch.full((8, c.rows, dim), 3.0, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    run_attention(gpu, c, q, dst, 0.1, impl)
+    s.wait()
+    check_attention(c, q, 0.1, dst, dst, "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
+def test_sequences_that_share_pages(gpu, impl):
+    """A common prefix, and the same sequence twice."""
+    torch, _ = T._torch()
+    c = Cache([200, 200, 200], [70, 70, 70], 2, 32, 64, "s8", seed=4)
+    t = c.np_table.copy()
+    t[1, :4] = t[0, :4]
+    t[2] = t[0]
+    c.np_table, c.table = t, torch.from_numpy(t).cuda()
+    q = torch.randn(c.rows, 4, 64, generator=c.g, device="cuda").to(torch.bfloat16)
+    dst = torch.full_like(q, math.nan)
+    run_attention(gpu, c, q, dst, 0.1, impl)
+    gpu[1].wait()
+    check_attention(c, q, 0.1, dst, dst, "bf16")
+
+
+@pytest.mark.gpu
+def test_many_sequences(gpu):
+    """Five thousand of them, most of one token, some without: append, read and attention find each row's."""
+    torch, types = T._torch()
+    e, s = gpu
+    n = 5000
+    lens = [1 + i * 7 % 23 for i in range(n)]
+    news = [0 if i % 11 == 0 else 1 for i in range(n)]
+    c = Cache(lens, news, 1, 8, 16, "s8", seed=6, behind=5)
+    x = torch.randn(c.rows, 1, 16, generator=c.g, device="cuda")
+    want = [T.expected_append(c, x, c.codes[i], c.scales[i]) for i in range(2)]
+    run_append(gpu, c, x, x)
+    s.wait()
+    for i in range(2):
+        assert torch.equal(c.scales[i], want[i][1]) and torch.equal(c.codes[i], want[i][0])
+    q = torch.randn(c.rows, 2, 16, generator=c.g, device="cuda").to(torch.bfloat16)
+    outs = []
+    for impl in (MMA, GENERIC):
+        dst = torch.full_like(q, 3.0)
+        run_attention(gpu, c, q, dst, 0.25, impl)
+        s.wait()
+        outs.append(dst)
+    kept = torch.full_like(q, 3.0)
+    check_attention(c, q, 0.25, outs[0], kept, "bf16")
+    check_attention(c, q, 0.25, outs[1], kept, "bf16")
+
+
+# ---- the norm's plans for many rows ----------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols,src,residual,gamma,dst", [
+    (300, 264, "bf16", "bf16", "f32", "s8"), (300, 512, "f16", "", "bf16", "f16"), (257, 1024, "bf16", "f32", "f32", "e4m3"),
+    (300, 1032, "f32", "bf16", "", "s8"), (300, 4096, "bf16", "bf16", "f32", "e4m3"), (270, 8192, "f16", "f32", "f16", "s8"),
+    (300, 5003, "bf16", "bf16", "f32", "s8"), (1031, 64, "f32", "", "f32", "s8"), (1025, 136, "bf16", "f16", "f32", "bf16")])
+def test_norm_of_many_rows(gpu, rows, cols, src, residual, gamma, dst):
+    torch, types = T._torch()
+    torch.manual_seed(rows + cols)
+    x = (torch.randn(rows, cols, device="cuda") * 3).to(types[src])
+    r = (torch.randn(rows, cols, device="cuda") * 5).to(types[residual]) if residual else None
+    g = (torch.rand(cols, device="cuda") + 0.5).to(types[gamma]) if gamma else None
+    out = torch.zeros(rows, cols, dtype=types[dst], device="cuda")
+    total, scales = T.run_norm(gpu, x, r, g, out, 1e-5)
+    T.check_norm(x, r, g, out, 1e-5, total, scales, dst)
