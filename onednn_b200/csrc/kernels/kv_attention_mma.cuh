@@ -14,8 +14,9 @@
 // FINE (f16 results): what a weight's rounding to f16 left is multiplied too; bf16's own last rounding is eight
 // times as large, so there it would not show.
 // Scales stay out of the products: the key's multiplies the score, the value's the weight.  f16 holds weight times
-// value scale, P = 2^(x - m - k + 14) * scale, with two numbers of each row: m, the largest score x that it has seen, and k, a
-// whole number such that no token that it sees has x + log2(scale) above m + k.  So P < 2^14, rounded to 2^-11 of
+// value scale, P = 2^(x - m - k + 14) * scale, with two numbers of each row: m, the largest score x that it has seen, and k, such
+// that no token that it sees has x + log2(scale) above m + k (k goes down as m goes up, exactly: rounded to whole numbers it
+// stayed, and scores that rose by less than 2 per step left m + k far above all that counted).  So P < 2^14, rounded to 2^-11 of
 // itself down to 2^-28 of that, and no page that a row does not see, or gives no weight, takes bits from the others.  In a
 // step whose scales lie within 2^4 of one another the largest stands for all; else k comes from the tokens one by one.
 // Sum and weighted values are both relative to 2^(m + k - 14).  Queries are taken to f16 after a power of two per row that
@@ -28,8 +29,8 @@
 #include <type_traits>
 
 //
-// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 120 us, e4m3 116 us (574 MB: 4.8
-// and 4.9 TB/s); one of 131009 tokens: 65 us (4.1 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
+// Measured on one B200: 64 sequences of 900 to 8100 tokens, 32 query heads on 8, dim 128: s8 120 us, e4m3 112 us (574 MB: 4.8
+// and 5.1 TB/s); one of 131009 tokens: 65 us (4.1 TB/s).  Some 900 instructions per 32 tokens and warp at 0.5 per
 // cycle and scheduler: three blocks of four warps per SM are what registers and rings allow (two blocks: 150 us), and
 // the loops wait for their own results more than for memory.
 namespace b200 {
@@ -83,8 +84,6 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// 2^n of a whole number -126 <= n <= 127
-__device__ __forceinline__ float pow2(float n) { return __uint_as_float(__float_as_uint(n + (8388608.f + 127.f)) << 23); }
 // to f16, at most its largest number: where scores are so large (2^25) that differences of them are whole numbers off
 __device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
     uint32_t r;
@@ -477,7 +476,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                     for (int h = 0; h < 2; ++h) {
                         // (fmaxf passes over the NaN of infinite scores, or of none)
                         const float less = m[nb][h] - now[nb][h];
-                        const float k = fminf(fmaxf(fmaxf(k2[nb][h] + ceilf(less), ceilf(rel[nb][h])), K_MIN), K_MAX);
+                        const float k = fminf(fmaxf(fmaxf(k2[nb][h] + less, rel[nb][h]), K_MIN), K_MAX);
                         fo[h] = now[nb][h] == -INFINITY ? 1.f : ex2(less + (k2[nb][h] - k));
                         l[nb][h] *= fo[h];
                         m[nb][h] = now[nb][h];
@@ -560,8 +559,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
         float *mine = (float *)ring;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const float up[2] = { // from here on relative to 2^m
-                    pow2(k2[nb][0] - P_TOP), pow2(k2[nb][1] - P_TOP)};
+            const float up[2] = {ex2(k2[nb][0] - P_TOP), ex2(k2[nb][1] - P_TOP)}; // from here on relative to 2^m
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll

@@ -20,14 +20,14 @@
 // The two scales stay out of the products.  A page holds a multiple of RUN (16 or 8) tokens here, so as many neighbouring tokens
 // share theirs: x = s * (key scale * softmax scale) in the exponent's multiply-add, P = w * value scale with
 // w = 2^(x - m - k + 14), two elements at a time, and the sum is of the w.  m and k are the row's own: m follows the largest
-// score that the row has seen when that has grown by more than 2^8, which saves most rescaling of O; k, a whole number, is
+// score that the row has seen when that has grown by more than 2^8, which saves most rescaling of O; k is
 // not below x + log2(value scale) - m of any token that the row sees.  So P < 2^14, rounded to f16 relative to what the row
 // sees, and no page that it does not see, or gives no weight, takes bits from the others (with the value scale in the
 // exponent, relative to the largest of all pages, 3 % faster, a page 2^30 above the others took them to zero in rows that
 // did not see it).  FINE (f16 results): what P's rounding left is multiplied too.
 //
 // Measured on one B200: three sequences with 1450, 1029 and 1710 new tokens on 5750, 4647 and 3543, 32 query heads on 8, dim 128, s8,
-// bf16: 340 us, 778 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
+// bf16: 338 us, 782 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
 // alone take 1.3.  What is left: a softmax step of 64 columns takes a warp 2000 cycles, two of the three warps on a
 // scheduler; items begin and end (8 us each) and cut ones are joined (10 us).  Not kept: 16 softmax warps, two threads per row
 // (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
@@ -235,8 +235,6 @@ __device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
     asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// 2^n of a whole number -126 <= n <= 127
-__device__ __forceinline__ float pow2(float n) { return __uint_as_float(__float_as_uint(n + (8388608.f + 127.f)) << 23); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -508,7 +506,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         float fo = 1.f;
                         if (follow) { // (fmaxf passes over the NaN of infinite scores)
                             const float now = fmaxf(m, top), less = m - now;
-                            const float k = fminf(fmaxf(fmaxf(k2 + ceilf(less), ceilf(rel + (from - now)) + ROOM), K_MIN), K_MAX);
+                            const float k = fminf(fmaxf(fmaxf(k2 + less, rel + (from - now) + ROOM), K_MIN), K_MAX);
                             fo = ex2(less + (k2 - k));
                             m = now, k2 = k;
                         }
@@ -575,7 +573,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
 
             // ---- the row's result, or its part of it
             const bool whole = seg->whole;
-            const float up = pow2(k2 - P_TOP); // O and l are relative to 2^(m + k - 14), parts to 2^m
+            const float up = ex2(k2 - P_TOP); // O and l are relative to 2^(m + k - 14), parts to 2^m
             if (l != l) m = INFINITY; // a NaN among the scores, which no maximum shows
             const int idx = seg->row0 + t * TILE + r;
             char *to = (char *)p.dst + ((int64_t)(seg->begin + idx / group) * p.dst_s0 + ((int64_t)seg->head * group + idx % group) * p.dst_s1) * 2;

@@ -167,6 +167,33 @@ def test_value_scales_of_pages_that_do_not_count(gpu, impl, kind, shape, what):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("impl,seqs,news", [(MMA, 64, 1), (MMA, 64, 3), (TC, 40, 48)])
+@pytest.mark.parametrize("rise", [0.7, 0.95, 8.9])
+def test_scores_that_rise_step_by_step_behind_a_large_page(gpu, impl, seqs, news, rise):
+    """A first page of large values and low scores, then pages whose scores rise by 2^rise each: in the end the first page has no
+    weight.  Whatever stood for it in a row's exponent is to be gone by then."""
+    torch, _ = T._torch()
+    page, pages, heads, dim = 128, 56, 8, 64
+    c = Cache([page * pages] * seqs, [news] * seqs, heads, page, dim, "s8", seed=8)
+    c.codes[0].zero_()
+    c.codes[0][..., 0] = 64
+    for b in range(seqs):
+        ids = torch.from_numpy(c.np_table[b].astype(np.int64)).cuda()
+        c.scales[0][ids] = (torch.arange(pages, device="cuda")[:, None] + 1) * (rise * math.log(2) / 64 / 0.125)
+        c.scales[1][ids[0]] *= 2.0 ** min(60, rise * 44)
+    q = torch.zeros(c.rows, heads, dim, device="cuda")
+    q[..., 0] = 1
+    q = q.to(torch.bfloat16)
+    dst = torch.full_like(q, math.nan)
+    run_attention(gpu, c, q, dst, 0.125, impl)
+    gpu[1].wait()
+    want, tol = closeness(c, q, 0.125, "bf16")
+    err = (dst.double() - want).abs()
+    assert not torch.isnan(dst).any()
+    assert (err <= tol).all(), "%g of the tolerance, %d of %d" % (float((err / tol).max()), int((err > tol).sum()), err.numel())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
 @pytest.mark.parametrize("kind", ["s8", "e4m3"])
 @pytest.mark.parametrize("page", [16, 24])
