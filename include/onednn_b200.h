@@ -383,7 +383,7 @@ dnnl_status_t DNNL_API dnnl_reorder_primitive_desc_create(dnnl_primitive_desc_t 
  *   WRITES to DNNL_ARG_ATTR_SCALES | DNNL_ARG_DST: f32, one per row -- what a matmul takes as its
  *   source scales with a mask over rows and one group over K.
  *   Arguments: DNNL_ARG_SRC, DNNL_ARG_SRC_1 (residual), DNNL_ARG_SCALE; DNNL_ARG_DST,
- *   DNNL_ARG_DST_1 (h rounded to the residual's type, same descriptor; may be the residual's own memory).
+ *   DNNL_ARG_DST_1 (h rounded to the residual's type, same descriptor; may be the residual's own memory, not DNNL_ARG_DST's).
  *
  * The cache: keys and values each of one descriptor (pages, heads, tokens per page, dim), s8 or
  *   f8_e4m3, with one f32 scale per page and head (DNNL_ARG_B200_KEY_SCALES / _VALUE_SCALES,
@@ -398,12 +398,14 @@ dnnl_status_t DNNL_API dnnl_reorder_primitive_desc_create(dnnl_primitive_desc_t 
  * dnnl_b200_kv_cache_append: keys DNNL_ARG_SRC and values DNNL_ARG_SRC_1, both src_desc (rows, heads,
  *   dim), f32 / bf16 / f16 -- slices of a matmul's result, say -- are quantised into the cache.  The
  *   scale of a page grows to what its tokens need, and the codes it held are then rounded again.
- *   Two sequences of one call may not write the same page.
+ *   Two sequences of one call may not write the same page.  Keys and values may not share places in
+ *   caches or scales (dnnl_invalid_arguments), but may lie in each other's gaps; nor may the two results of a read.
  * dnnl_b200_kv_cache_read: the inverse; DNNL_ARG_DST and DNNL_ARG_DST_1 of dst_desc (rows, heads, dim).
  * dnnl_b200_kv_cache_attention: DNNL_ARG_SRC, the queries (rows, q heads, dim), q heads a multiple
  *   of the cache's heads, attend to the tokens of their sequence up to their own;
  *   DNNL_ARG_DST the same dims.  dim at most 256.  softmax_scale multiplies query . key.  A row
- *   that sees no token is zero.  Different executions of one primitive must not overlap in time
+ *   that sees no token is zero.  What is rounded to f16 on the way, and relative to what: b200_kv_attention_params_t
+ *   in onednn_b200_kernels.h.  Different executions of one primitive must not overlap in time
  *   unless the scratchpad is the user's (DNNL_ARG_SCRATCHPAD); a captured execution has one of its own. */
 dnnl_status_t DNNL_API dnnl_b200_rms_norm_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
         dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc,

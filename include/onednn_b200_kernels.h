@@ -310,7 +310,8 @@ B200_API int b200_rms_norm_launch(const b200_rms_norm_params_t *p, b200_stream_t
  * its last tokens: with n = offsets[b + 1] - offsets[b], row offsets[b] + i is token
  * lens[b] - n + i.  Rows of no sequence are neither read nor written.
  * A page index outside 0 .. pages - 1, or a token beyond the table, is never accessed: the
- * kernels OR B200_STATUS_BAD_PAGE into *status and carry on without that token. */
+ * kernels OR B200_STATUS_BAD_PAGE into *status and carry on without that token.  *status is written when a kernel
+ * runs: of a captured launch, whenever its graph does. */
 #define B200_STATUS_BAD_PAGE 0x40000000u
 typedef struct {
     void *key, *value;
@@ -346,7 +347,16 @@ B200_API int b200_kv_read_launch(const b200_kv_rows_params_t *p, b200_stream_t s
 /* Attention of each sequence's last tokens over its cache:
  *   dst[row][j] = sum_t p[t] * v[t] / sum_t p[t],  p[t] = exp(scale * q[row][j] . k[t])
  * over the tokens t up to the row's own, with the keys and values of head j / (q_heads / heads).
- * A row that sees no token is zero.  Sums, maxima and exponentials in f32. */
+ * A row that sees no token is zero.  Scores, sums, maxima and exponentials in f32.
+ * The generic kernel rounds nothing else before the result.  The other two have f16 operands for their matrix products:
+ *   queries, after a power of two per row that brings its largest element to [1, 2): exact down to 2^-14 (bf16: 2^-17) of
+ *     the largest, in steps of 2^-24 of it below;
+ *   weights p[t] * value scale, to 2^-11 of each down to 2^-14 of the largest that the row itself has at a token it sees,
+ *     in steps of 2^-24 of that below.  f16 results: what that rounding left is multiplied too, 2^-22.  Tokens that a row does not see,
+ *     or gives no weight, have no part in this, whatever their scales.
+ * Value scales are positive normal numbers.  Where all that a row sees are below 2^-70 (values below 2^-63), its weights lose bits
+ * next to 2^-70, below 2^-105 all.
+ * Tokens from 2^31 - 256 on count as beyond the table. */
 typedef struct {
     b200_kv_cache_t cache;
     const void *query; int32_t query_dt; int32_t reserved0; int64_t query_s0, query_s1;

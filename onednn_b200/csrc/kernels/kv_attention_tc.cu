@@ -27,7 +27,7 @@
 // did not see it).  FINE (f16 results): what P's rounding left is multiplied too.
 //
 // Measured on one B200: three sequences with 1450, 1029 and 1710 new tokens on 5750, 4647 and 3543, 32 query heads on 8, dim 128, s8,
-// bf16: 338 us, 782 Tflop/s of the pairs that causality leaves; 2.5 us per 128 tokens and 256 rows, where the MMAs
+// bf16: 338 us, 782 Tflop/s of the pairs that causality leaves; 2.6 us per 128 tokens and 256 rows, where the MMAs
 // alone take 1.3.  What is left: a softmax step of 64 columns takes a warp 2000 cycles, two of the three warps on a
 // scheduler; items begin and end (8 us each) and cut ones are joined (10 us).  Not kept: 16 softmax warps, two threads per row
 // (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
@@ -953,8 +953,8 @@ extern "C" B200_API int b200_kv_attention_tc_supported(const b200_kv_attention_p
     // what the other kernel takes, with pages of whole runs of 8 tokens
     if (!b200_kv_attention_mma_supported(p) || p->cache.dim > 128 || p->cache.page % 8) return 0;
     // and at least 48 query rows per sequence and key head: a tile costs the same however many of its rows there are.  16
-    // sequences of 700 to 4500 tokens, 8 query heads on each of 5 key heads: 32 rows take 50 us there and 61 here, 48 rows 61 and
-    // 62, 64 rows 74 and 62, 128 rows 130 and 62.
+    // sequences of 700 to 4500 tokens, 8 query heads on each of 5 key heads: 32 rows take 52 us there and 64 here, 48 rows 62 and
+    // 64, 64 rows 76 and 64, 128 rows 134 and 64.
     return p->cache.seqs > 0 && p->cache.heads > 0 && p->rows / p->cache.seqs * (p->q_heads / p->cache.heads) >= 48;
 }
 
