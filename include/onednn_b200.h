@@ -406,7 +406,7 @@ dnnl_status_t DNNL_API dnnl_reorder_primitive_desc_create(dnnl_primitive_desc_t 
  *   DNNL_ARG_DST the same dims.  dim at most 256.  softmax_scale multiplies query . key.  A row
  *   that sees no token is zero.  What is rounded to f16 on the way, and relative to what: b200_kv_attention_params_t
  *   in onednn_b200_kernels.h.  Different executions of one primitive must not overlap in time
- *   unless the scratchpad is the user's (DNNL_ARG_SCRATCHPAD); a captured execution has one of its own. */
+ *   unless the scratchpad is the user's (DNNL_ARG_SCRATCHPAD, one for each under way); a captured execution has one of its own. */
 dnnl_status_t DNNL_API dnnl_b200_rms_norm_primitive_desc_create(dnnl_primitive_desc_t *primitive_desc,
         dnnl_engine_t engine, const_dnnl_memory_desc_t src_desc, const_dnnl_memory_desc_t residual_desc,
         const_dnnl_memory_desc_t scale_desc, const_dnnl_memory_desc_t dst_desc, float epsilon,

@@ -23,6 +23,7 @@
 // brings the largest element to [1, 2).
 #pragma once
 
+#include "kv_f16.cuh"
 #include "kv_line.cuh"
 #include "launch.hpp"
 
@@ -66,7 +67,6 @@ inline size_t part_floats(int dp, int nb) { return (size_t)8 * nb * (dp + 2); }
 
 // ---- small pieces -------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
@@ -79,42 +79,9 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// to f16, at most its largest number: where scores are so large (2^25) that differences of them are whole numbers off
-__device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 // a whole number above the base-2 logarithm of a value with these bits, by one at most
 __device__ __forceinline__ float above_log2(uint32_t bits) { return (float)((int)(bits >> 23) - 126); }
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t v) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-    return r;
-}
-// four codes -> two f16 pairs, exactly.  s8: code + 128 in the low byte of 0x6400 (1024), minus 1152.
-template <bool S8>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if (S8) {
-        w ^= 0x80808080u;
-        lo = hsub2(prmt(w, 0x64646464u, 0x4140), 0x64806480u);
-        hi = hsub2(prmt(w, 0x64646464u, 0x4342), 0x64806480u);
-    } else {
-        lo = e4m3x2_f16x2((uint16_t)w);
-        hi = e4m3x2_f16x2((uint16_t)(w >> 16));
-    }
-}
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])

@@ -33,6 +33,7 @@
 // (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
 //
 // Every wait is bounded; one that runs out sets a bit in the stream's status word and all roles leave.
+#include "kv_f16.cuh"
 #include "kv_line.cuh"
 #include "launch.hpp"
 
@@ -100,7 +101,6 @@ struct ctrl_t {
     int64_t line_words[LINE_WORDS];
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
 }
@@ -224,17 +224,6 @@ __device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lead, uin
     return (uint64_t)((saddr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46
             | (uint64_t)2 << 61;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// to f16, at most its largest number: where scores are so large (2^25) that differences of them are whole numbers off
-__device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -264,20 +253,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-// four codes -> two f16 pairs, exactly (s8: code + 128 in the low byte of 1024, minus 1152)
-template <bool S8>
-__device__ __forceinline__ uint2 widen(uint32_t w) {
-    uint2 r;
-    if (S8) {
-        w ^= 0x80808080u;
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(__byte_perm(w, 0x64646464u, 0x4140)), "r"(0x64806480u));
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(__byte_perm(w, 0x64646464u, 0x4342)), "r"(0x64806480u));
-    } else {
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r.x) : "h"((uint16_t)w));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r.y) : "h"((uint16_t)(w >> 16)));
-    }
     return r;
 }
 // f16 tiles: [block of 64 dims][row][128 bytes], 16-byte pieces swizzled by the row
@@ -735,9 +710,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
                     const int row = w * 32 + i * PER + sub_row;
-                    const uint2 a = widen<S8>(regs[i].x), b = widen<S8>(regs[i].y), d = widen<S8>(regs[i].z), e = widen<S8>(regs[i].w);
-                    *(uint4 *)(to + piece_at(row, cc * 2)) = make_uint4(a.x, a.y, b.x, b.y);
-                    *(uint4 *)(to + piece_at(row, cc * 2 + 1)) = make_uint4(d.x, d.y, e.x, e.y);
+                    uint4 a, b;
+                    widen<S8>(regs[i].x, a.x, a.y);
+                    widen<S8>(regs[i].y, a.z, a.w);
+                    widen<S8>(regs[i].z, b.x, b.y);
+                    widen<S8>(regs[i].w, b.z, b.w);
+                    *(uint4 *)(to + piece_at(row, cc * 2)) = a;
+                    *(uint4 *)(to + piece_at(row, cc * 2 + 1)) = b;
                 }
             };
             // keys of unit j (the i-th since the launch), and both scales: a softmax that sees the scores sees them
@@ -953,8 +932,8 @@ extern "C" B200_API int b200_kv_attention_tc_supported(const b200_kv_attention_p
     // what the other kernel takes, with pages of whole runs of 8 tokens
     if (!b200_kv_attention_mma_supported(p) || p->cache.dim > 128 || p->cache.page % 8) return 0;
     // and at least 48 query rows per sequence and key head: a tile costs the same however many of its rows there are.  16
-    // sequences of 700 to 4500 tokens, 8 query heads on each of 5 key heads: 32 rows take 52 us there and 64 here, 48 rows 62 and
-    // 64, 64 rows 76 and 64, 128 rows 134 and 64.
+    // sequences of 700 to 4500 tokens, 8 query heads on each of 5 key heads: there 32 rows take 52 us, 48 62, 64 76, 128 134;
+    // here 48 to 128 take 64.
     return p->cache.seqs > 0 && p->cache.heads > 0 && p->rows / p->cache.seqs * (p->q_heads / p->cache.heads) >= 48;
 }
 
