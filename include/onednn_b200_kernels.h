@@ -354,8 +354,8 @@ B200_API int b200_kv_read_launch(const b200_kv_rows_params_t *p, b200_stream_t s
  *   weights p[t] * value scale, to 2^-11 of each down to 2^-14 of the largest that the row itself has at a token it sees,
  *     in steps of 2^-24 of that below.  f16 results: what that rounding left is multiplied too, 2^-22.  Tokens that a row does not see,
  *     or gives no weight, have no part in this, whatever their scales.
- * Value scales are positive normal numbers.  Where all that a row sees are below 2^-70 (values below 2^-63), its weights lose bits
- * next to 2^-70, below 2^-105 all.
+ * Value scales are positive normal numbers; where all that a row sees are below 2^-100, its weights lose f16's last bits.
+ * The tcgen05 kernel takes scores, times log2 e, up to 2^26 in magnitude: a row whose largest is beyond is NaN.
  * Tokens from 2^31 - 256 on count as beyond the table. */
 typedef struct {
     b200_kv_cache_t cache;

@@ -14,12 +14,12 @@
 // FINE (f16 results): what a weight's rounding to f16 left is multiplied too; bf16's own last rounding is eight
 // times as large, so there it would not show.
 // Scales stay out of the products: the key's multiplies the score, the value's the weight.  f16 holds weight times
-// value scale, P = 2^(x - m - k + 14) * scale, with two numbers of each row: m, the largest score x that it has seen, and k, such
+// value scale, P = 2^(x - m) * 2^(14 - k) * scale, with two numbers of each row: m, the largest score x that it has seen, and k, such
 // that no token that it sees has x + log2(scale) above m + k (k goes down as m goes up, exactly: rounded to whole numbers it
 // stayed, and scores that rose by less than 2 per step left m + k far above all that counted).  So P < 2^14, rounded to 2^-11 of
 // itself down to 2^-28 of that, and no page that a row does not see, or gives no weight, takes bits from the others.  In a
 // step whose scales lie within 2^4 of one another the largest stands for all; else k comes from the tokens one by one.
-// Sum and weighted values are both relative to 2^(m + k - 14).  Queries are taken to f16 after a power of two per row that
+// The sum is relative to 2^m, the weighted values to 2^(m + k - 14).  Queries are taken to f16 after a power of two per row that
 // brings the largest element to [1, 2).
 #pragma once
 
@@ -42,8 +42,7 @@ using namespace kv_line;
 constexpr int EXTRA = 1; // units that an item's queries and result take besides
 constexpr int WARPS = 4, THREADS = WARPS * 32, STEP = 32;
 constexpr float P_TOP = 14.f; // weights in f16 stay below 2^14
-// of k: the sum, relative to 2^(m + k - 14), holds 2^31 tokens.  Where all scales that a row sees are below 2^-80, f16's last bits go unused
-constexpr float K_MIN = -80.f, K_MAX = 121.f;
+constexpr float K_MIN = -100.f, K_MAX = 121.f; // of k: where all scales that a row sees are below 2^-100, f16's last bits go unused
 static_assert(WARPS * STEP == UNIT, "a warp takes one step of each unit");
 
 // blocks per SM
@@ -445,7 +444,7 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                         const float less = m[nb][h] - now[nb][h];
                         const float k = fminf(fmaxf(fmaxf(k2[nb][h] + less, rel[nb][h]), K_MIN), K_MAX);
                         fo[h] = now[nb][h] == -INFINITY ? 1.f : ex2(less + (k2[nb][h] - k));
-                        l[nb][h] *= fo[h];
+                        l[nb][h] *= now[nb][h] == -INFINITY ? 1.f : ex2(less);
                         m[nb][h] = now[nb][h];
                         k2[nb][h] = k;
                     }
@@ -465,19 +464,19 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
                 uint32_t pb[NB][2], rest[NB][2];
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    const float m0 = (m[nb][0] == -INFINITY ? 0.f : m[nb][0]) + (k2[nb][0] - P_TOP);
-                    const float m1 = (m[nb][1] == -INFINITY ? 0.f : m[nb][1]) + (k2[nb][1] - P_TOP);
+                    const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+                    const float r0 = ex2(P_TOP - k2[nb][0]), r1 = ex2(P_TOP - k2[nb][1]);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float w0 = ex2(st[tt][nb][i * 2] - m0), w1 = ex2(st[tt][nb][i * 2 + 1] - m1);
                         l[nb][0] += w0;
                         l[nb][1] += w1;
-                        const float p0 = w0 * vs[tt * 2 + i], p1 = w1 * vs[tt * 2 + i];
-                        const uint32_t hi = pack_held_f16x2(p0, p1);
+                        const float p0 = w0 * r0 * vs[tt * 2 + i], p1 = w1 * r1 * vs[tt * 2 + i]; // in this order: no weight times a large scale is 0
+                        const uint32_t hi = pack_f16x2(p0, p1);
                         pb[nb][i] = transposed(hi);
                         if (FINE) {
                             const float2 had = f16x2_to_f32(hi);
-                            rest[nb][i] = transposed(pack_held_f16x2(p0 - had.x, p1 - had.y));
+                            rest[nb][i] = transposed(pack_f16x2(p0 - had.x, p1 - had.y));
                         }
                     }
                 }
@@ -531,7 +530,6 @@ kv_attention_mma_kernel(const __grid_constant__ b200_kv_attention_params_t p) {
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) l[nb][h] += __shfl_xor_sync(~0u, l[nb][h], w);
-                l[nb][h] *= up[h];
                 // a NaN among the scores, which no maximum shows, is to be the row's result
                 if (l[nb][h] != l[nb][h]) m[nb][h] = INFINITY;
                 if (g == 0) merge_m[warp][nb * 8 + 2 * t + h] = m[nb][h], merge_l[warp][nb * 8 + 2 * t + h] = l[nb][h];

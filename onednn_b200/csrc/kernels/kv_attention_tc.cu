@@ -18,16 +18,16 @@
 //   warp 14          finds the block's items ahead of all others and lays them out in shared memory
 //
 // The two scales stay out of the products.  A page holds a multiple of RUN (16 or 8) tokens here, so as many neighbouring tokens
-// share theirs: x = s * (key scale * softmax scale) in the exponent's multiply-add, P = w * value scale with
-// w = 2^(x - m - k + 14), two elements at a time, and the sum is of the w.  m and k are the row's own: m follows the largest
+// share theirs: x = s * (key scale * softmax scale) in the exponent's multiply-add, P = w * (value scale * 2^(13 - k)) with
+// w = 2^(x - m), two elements at a time, and the sum is of the w.  m and k are the row's own: m follows the largest
 // score that the row has seen when that has grown by more than 2^8, which saves most rescaling of O; k is
-// not below x + log2(value scale) - m of any token that the row sees.  So P < 2^14, rounded to f16 relative to what the row
+// not below x + log2(value scale) - m of any token that the row sees.  So P < 2^13, rounded to f16 relative to what the row
 // sees, and no page that it does not see, or gives no weight, takes bits from the others (with the value scale in the
 // exponent, relative to the largest of all pages, 3 % faster, a page 2^30 above the others took them to zero in rows that
 // did not see it).  FINE (f16 results): what P's rounding left is multiplied too.
 //
 // Measured on one B200: three sequences with 1450, 1029 and 1710 new tokens on 5750, 4647 and 3543, 32 query heads on 8, dim 128, s8,
-// bf16: 338 us, 782 Tflop/s of the pairs that causality leaves; 2.6 us per 128 tokens and 256 rows, where the MMAs
+// bf16: 342 us, 772 Tflop/s of the pairs that causality leaves; 2.6 us per 128 tokens and 256 rows, where the MMAs
 // alone take 1.3.  What is left: a softmax step of 64 columns takes a warp 2000 cycles, two of the three warps on a
 // scheduler; items begin and end (8 us each) and cut ones are joined (10 us).  Not kept: 16 softmax warps, two threads per row
 // (3.6 us per 128 tokens: the converters lost their turns), 8 converter warps (3.6), one issuing thread (2.9).
@@ -69,10 +69,13 @@ struct scales_t {
     float4 chunk[UNIT / 8];
     float above, below; // whole numbers, not below and not above any log2(value scale)
 };
-constexpr float P_TOP = 14.f; // P stays below 2^14
+constexpr float P_TOP = 13.f; // P stays below 2^13
+// of m: x - m in one multiply-add leaves what rounding took from m, at most 2^2 up to here, for which P has room; rows beyond are NaN
+// (rounding x first, an operation more per element, has no such end and took 353 us instead of 341)
+constexpr float M_MOST = 67108864.f;
 constexpr float ROOM = 8.f;   // what m, and with it k, may lag behind
-// of k: the sum, relative to 2^(m + k - 14), holds 2^31 tokens.  Where all scales that a row sees are below 2^-70, f16's last bits go unused
-constexpr float K_MIN = -70.f, K_MAX = 121.f;
+constexpr float K_MIN = -100.f, K_MAX = 121.f; // of k: where all scales that a row sees are below 2^-100, f16's last bits go unused
+constexpr float G_MAX = 1.3292280e36f;         // 2^120, of the factor of a run that a row does not see: 0 * infinity is no weight
 constexpr float SMALL = 1.0842022e-19f; // 2^-63
 
 // a stretch of an item's tokens: what one block does of it
@@ -478,14 +481,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     }
                     const bool follow = top > m + ROOM || rel > k2; // also from -inf
                     if (__any_sync(~0u, follow)) {
-                        float fo = 1.f;
+                        float fo = 1.f, d = 1.f;
                         if (follow) { // (fmaxf passes over the NaN of infinite scores)
                             const float now = fmaxf(m, top), less = m - now;
                             const float k = fminf(fmaxf(fmaxf(k2 + less, rel + (from - now) + ROOM), K_MIN), K_MAX);
-                            fo = ex2(less + (k2 - k));
+                            d = fabsf(now) > M_MOST ? NAN : ex2(less), fo = ex2(less + (k2 - k));
                             m = now, k2 = k;
                         }
-                        l *= fo;
+                        l *= d;
                         if (j > 0) { // the products of the step before are added up first
                             if (!(ok = products_done(place ^ 1))) break;
                             tc_fence_after();
@@ -500,14 +503,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         }
                     }
                     // ---- weights, over the scores: of each 16 columns the first eight, FINE: the other eight too
-                    const float base = (m == -INFINITY ? 0.f : m) + (k2 - P_TOP);
+                    const float base = m == -INFINITY ? 0.f : m, unit = ex2(P_TOP - k2);
 #pragma unroll
                     for (int h = 0; h < STEP / 16; ++h) {
                         uint32_t pw[FINE ? 16 : 8];
 #pragma unroll
                         for (int k = h * 16 / RUN; k < (h + 1) * 16 / RUN; ++k) {
                             const uint32_t *y = v[k * RUN >> 5] + (k * RUN & 31);
-                            const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(ck[k].y - base, ck[k].y - base), vv = f32x2(ck[k].w, ck[k].w);
+                            const float g = min_nan(ck[k].w * unit, G_MAX);
+                            const uint64_t ff = f32x2(f[k], f[k]), oo = f32x2(ck[k].y - base, ck[k].y - base), vv = f32x2(g, g);
                             uint64_t sum = 0;
 #pragma unroll
                             for (int i = 0; i < RUN; i += 2) {
@@ -516,11 +520,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                                 const float e0 = ex2(x.x), e1 = ex2(x.y);
                                 sum = add2(sum, f32x2(e0, e1));
                                 const float2 pv = unpack2(mul2(f32x2(e0, e1), vv));
-                                const uint32_t hi = pack_held_f16x2(pv.x, pv.y);
+                                const uint32_t hi = pack_f16x2(pv.x, pv.y);
                                 pw[at] = hi;
                                 if (FINE) {
                                     const float2 had = f16x2_to_f32(hi);
-                                    pw[FINE ? 8 + at : 0] = pack_held_f16x2(pv.x - had.x, pv.y - had.y);
+                                    pw[FINE ? 8 + at : 0] = pack_f16x2(pv.x - had.x, pv.y - had.y);
                                 }
                             }
                             const float2 both = unpack2(sum);
@@ -548,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
 
             // ---- the row's result, or its part of it
             const bool whole = seg->whole;
-            const float up = ex2(k2 - P_TOP); // O and l are relative to 2^(m + k - 14), parts to 2^m
+            const float up = ex2(k2 - P_TOP); // O is relative to 2^(m + k - 13), parts, as l, to 2^m
             if (l != l) m = INFINITY; // a NaN among the scores, which no maximum shows
             const int idx = seg->row0 + t * TILE + r;
             char *to = (char *)p.dst + ((int64_t)(seg->begin + idx / group) * p.dst_s0 + ((int64_t)seg->head * group + idx % group) * p.dst_s1) * 2;
@@ -573,20 +577,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                         for (int i = 0; i < 32; i += 8) {
                             float x[8];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]);
+                            for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(v[i + k]) * up;
                             if (whole) {
                                 put(h * 32 + i, x, inv);
                             } else { // rows side by side, so that a warp's stores are contiguous
                                 float4 *d4 = (float4 *)(part + 2 * ROWS) + (h * 32 + i) / 4 * ROWS + pr;
-                                d4[0] = make_float4(x[0] * up, x[1] * up, x[2] * up, x[3] * up);
-                                d4[ROWS] = make_float4(x[4] * up, x[5] * up, x[6] * up, x[7] * up);
+                                d4[0] = make_float4(x[0], x[1], x[2], x[3]);
+                                d4[ROWS] = make_float4(x[4], x[5], x[6], x[7]);
                             }
                         }
                     }
                     __syncwarp(); // the next load is the whole warp's, lanes without a row among them
                 }
                 tc_fence_before(); // O may be written again after the next arrival
-                if (!whole && mine) part[pr] = m, part[ROWS + pr] = l * up;
+                if (!whole && mine) part[pr] = m, part[ROWS + pr] = l;
             }
             if (!whole && ok) {
                 // an item in several parts: the last block to finish one puts them together, in the order of the parts

@@ -11,10 +11,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// to f16, at most its largest number: where scores are so large (2^25) that differences of them are whole numbers off
-__device__ __forceinline__ uint32_t pack_held_f16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+__device__ __forceinline__ float min_nan(float a, float b) { // keeps a NaN
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {

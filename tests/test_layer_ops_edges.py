@@ -195,6 +195,43 @@ def test_scores_that_rise_step_by_step_behind_a_large_page(gpu, impl, seqs, news
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
+@pytest.mark.parametrize("scale", [1e3, -1e3, 1e6, -1e7, 2e7, 1e9, 1e15, 1e30])
+@pytest.mark.parametrize("large", [1.0, 2.0 ** 30])
+def test_scores_of_any_size(gpu, impl, scale, large):
+    """Every token a key of its own: the row's result is the value of the best one that it sees, however large scores are.  One
+    weight, rounded to f16, then the result's rounding.  The prompts' kernel takes scores, times log2 e, to
+    2^26 (here scale * 127 / 8 * log2 e); a row beyond is NaN, none is wrong."""
+    torch, _ = T._torch()
+    lens, news = [250, 130], [100, 60]
+    c = Cache(lens, news, 1, 32, 64, "s8", seed=9)
+    q = torch.zeros(c.rows, 1, 64, device="cuda")
+    q[..., 0] = 1
+    q = q.to(torch.bfloat16)
+    c.codes[0].zero_()
+    c.scales[0].fill_(0.125)
+    c.scales[1][1::2] *= large
+    want = torch.zeros(c.rows, 64, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(lens):
+        key = torch.randperm(255, generator=c.g, device="cuda")[:n] - 127
+        ids = torch.from_numpy(c.np_table[b, :-(-n // 32)].astype(np.int64)).cuda()
+        page = torch.zeros(len(ids) * 32, dtype=torch.int8, device="cuda")
+        page[:n] = key.to(torch.int8)
+        c.codes[0][ids, 0, :, 0] = page.view(-1, 32)
+        value = c.dense(1, b, n)[:, 0]
+        for i in range(news[b]):
+            seen = n - news[b] + i + 1
+            want[int(c.np_off[b]) + i] = value[int((key[:seen] * (1 if scale > 0 else -1)).argmax())]
+    dst = torch.full_like(q, math.nan)
+    run_attention(gpu, c, q, dst, scale, impl)
+    gpu[1].wait()
+    right = (dst[:, 0].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20)
+    if impl == TC and abs(scale) * 127 / 8 * 1.4427 > 2.0 ** 26:
+        right |= torch.isnan(dst[:, 0])
+    assert right.all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
 @pytest.mark.parametrize("kind", ["s8", "e4m3"])
 @pytest.mark.parametrize("page", [16, 24])
 def test_f16_results_come_from_unrounded_weights(gpu, impl, kind, page):
