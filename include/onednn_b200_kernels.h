@@ -351,11 +351,11 @@ B200_API int b200_kv_read_launch(const b200_kv_rows_params_t *p, b200_stream_t s
  * The generic kernel rounds nothing else before the result.  The other two have f16 operands for their matrix products:
  *   queries, after a power of two per row that brings its largest element to [1, 2): exact down to 2^-14 (bf16: 2^-17) of
  *     the largest, in steps of 2^-24 of it below;
- *   weights p[t] * value scale, to 2^-11 of each down to 2^-14 of the largest that the row itself has at a token it sees,
- *     in steps of 2^-24 of that below.  f16 results: what that rounding left is multiplied too, 2^-22.  Tokens that a row does not see,
+ *   weights p[t] * value scale, to 2^-11 of each down to 2^-13 of the largest that the row itself has at a token it sees,
+ *     in steps of 2^-23 of that below.  f16 results: what that rounding left is multiplied too, 2^-22.  Tokens that a row does not see,
  *     or gives no weight, have no part in this, whatever their scales.
  * Value scales are positive normal numbers; where all that a row sees are below 2^-100, its weights lose f16's last bits.
- * The tcgen05 kernel takes scores, times log2 e, up to 2^26 in magnitude: a row whose largest is beyond is NaN.
+ * The tcgen05 kernel takes scores, times log2 e, up to 2^26 in magnitude: a row with larger ones is right or NaN.
  * Tokens from 2^31 - 256 on count as beyond the table. */
 typedef struct {
     b200_kv_cache_t cache;

@@ -70,7 +70,8 @@ struct scales_t {
     float above, below; // whole numbers, not below and not above any log2(value scale)
 };
 constexpr float P_TOP = 13.f; // P stays below 2^13
-// of m: x - m in one multiply-add leaves what rounding took from m, at most 2^2 up to here, for which P has room; rows beyond are NaN
+// of m: x - m in one multiply-add leaves what rounding took from m, at most 2^2 up to here, for which P has room; a row whose m
+// goes beyond becomes NaN
 // (rounding x first, an operation more per element, has no such end and took 353 us instead of 341)
 constexpr float M_MOST = 67108864.f;
 constexpr float ROOM = 8.f;   // what m, and with it k, may lag behind
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv_attention_tc_kernel(const __gri
                     // ---- m and k follow, seldom; O and the sum with them.  `rel`: the largest x + log2(value scale) of the step, less
                     // m (differences first, so that scores of any size keep them).  Runs of 8, twice as many, are looked at one by
                     // one where their scales are further than 2^4 apart, else the largest stands for all (24 tokens per page: 345 us, each
-                    // time 350; with runs of 16 the branch costs as much as it saves: 340, without 338)
+                    // time 350; with runs of 16 the branch costs more than it saves: 340, without 338)
                     const float from = m == -INFINITY ? top : m;
                     float rel = (top - from) + sc.above;
                     if (RUN == 16 || sc.above - sc.below > 5.f) {
