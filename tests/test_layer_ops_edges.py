@@ -492,3 +492,57 @@ def test_norm_of_many_rows(gpu, rows, cols, src, residual, gamma, dst):
     out = torch.zeros(rows, cols, dtype=types[dst], device="cuda")
     total, scales = T.run_norm(gpu, x, r, g, out, 1e-5)
     T.check_norm(x, r, g, out, 1e-5, total, scales, dst)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("impl", [MMA, TC, GENERIC])
+@pytest.mark.parametrize("group,news", [(130, [1, 1]), (71, [1, 3]), (33, [2, 0])])
+def test_many_query_heads_on_one_key_head(gpu, impl, group, news):
+    torch, _ = T._torch()
+    c = Cache([300, 41], news, 1, 16, 64, "s8", seed=group)
+    q = torch.randn(c.rows, group, 64, generator=c.g, device="cuda").to(torch.bfloat16)
+    dst = torch.full_like(q, math.nan)
+    run_attention(gpu, c, q, dst, 0.125, impl)
+    gpu[1].wait()
+    check_attention(c, q, 0.125, dst, dst, "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 20])
+def test_read_with_more_rows_than_tokens(gpu, dim):
+    """Rows that stand for tokens before a sequence's first are zero, the others its tokens."""
+    torch, _ = T._torch()
+    e, s = gpu
+    c = Cache([3, 0, 9], [5, 2, 9], 2, 8, dim, "s8", behind=2)
+    out = torch.full((2, c.rows, 2, dim), 7.0, device="cuda")
+    p = api.Primitive(api.kv_cache_read_primitive_desc(e, tmd(c.codes[0]), tmd(out[0]), tmd(c.table)))
+    p.execute(s, {**c.args(e), api.ARG_DST: mem(out[0], e), api.ARG_DST_1: mem(out[1], e)})
+    s.wait()
+    for i in range(2):
+        assert (out[i, :2] == 0).all() and (out[i, 5:7] == 0).all() and (out[i, 16:] == 7).all()
+        for rows, b, n in ((slice(2, 5), 0, 3), (slice(7, 16), 2, 9)):
+            assert torch.equal(out[i, rows], c.dense(i, b, n).float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(7, 128), (300, 512), (5, 4096), (3, 257), (2, 20000)])
+def test_norm_in_the_memory_of_its_inputs(gpu, rows, cols):
+    """The sum written over src, and the result over src: each element is read before anything is written in its place."""
+    torch, _ = T._torch()
+    e, s = gpu
+    torch.manual_seed(cols)
+    x = torch.randn(rows, cols, device="cuda").to(torch.bfloat16)
+    r = torch.randn(rows, cols, device="cuda").to(torch.bfloat16)
+    for over in ("sum", "result"):
+        src, codes, scales = x.clone(), torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+        if over == "sum":
+            p = api.Primitive(api.rms_norm_primitive_desc(e, tmd(x), tmd(codes), 1e-5, residual_md=tmd(r)))
+            p.execute(s, {api.ARG_SRC: mem(src, e), api.ARG_SRC_1: mem(r, e), api.ARG_DST_1: mem(src, e), api.ARG_DST: mem(codes, e),
+                          api.ARG_ATTR_SCALES | api.ARG_DST: mem(scales, e)})
+            s.wait()
+            T.check_norm(x, r, None, codes, 1e-5, src, scales, "s8")
+        else:
+            p = api.Primitive(api.rms_norm_primitive_desc(e, tmd(x), tmd(x), 1e-5))
+            p.execute(s, {api.ARG_SRC: mem(src, e), api.ARG_DST: mem(src, e)})
+            s.wait()
+            T.check_norm(x, None, None, src, 1e-5, None, None, "bf16")
